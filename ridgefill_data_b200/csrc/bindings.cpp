@@ -88,6 +88,7 @@ bool set_gemm_2sm(bool on) {
 }  // namespace
 
 void register_ops(pybind11::module_& m);   // bind_ops.cpp
+void register_kv4(pybind11::module_& m);   // bind_kv4.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "ridgefill_data_b200 sm_100a kernels";
@@ -159,4 +160,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("residual") = py::none(), py::arg("epi") = 0, py::arg("bn") = 256, py::arg("a_mn") = false,
         py::arg("b_mn") = false, py::arg("k_splits") = 1, py::arg("k_chunk") = 0, py::arg("max_ctas") = 0);
   register_ops(m);
+  register_kv4(m);
 }

@@ -241,3 +241,102 @@ def router_topk(logits, k, norm_topk=True):
     if norm_topk:
         w = w / w.sum(-1, keepdim=True)
     return w, idx
+
+
+# ------------------------------------------------------------------------------ 4-bit K/V cache (ops/kv4.py)
+
+KV4_MARK = 255       # exponent byte of a row whose values are NaN
+
+
+def kv4_quantise(y):
+    """Rows y [..., hd] of bf16 values -> (exponent byte [...], s, m [..., hd / 32], codes [..., hd / 32, 32]), in fp32
+    with the cache's roundings: z = y 2^-e, m = fp16(min z), s = fp16((max z - min z) / 15), c = round((z - m) / s)."""
+    y = y.float()
+    top = y.abs().amax(-1)
+    bad = ~(top < 2.0 ** 56)
+    e = (torch.frexp(torch.where(bad | (top == 0), torch.ones_like(top), top))[1] - 1).clamp(-40, 40)
+    z = torch.where(bad[..., None], torch.zeros_like(y), y) * torch.pow(2.0, -e.double()).float()[..., None]
+    z = z.unflatten(-1, (-1, 32))
+    low, high = z.amin(-1), z.amax(-1)
+    m, s = low.half().float(), ((high - low) / 15).half().float()
+    c = torch.round((z - m[..., None]) / torch.where(s == 0, torch.ones_like(s), s)[..., None]).clamp(0, 15)
+    c = torch.where(s[..., None] == 0, torch.zeros_like(c), c)
+    return torch.where(bad, torch.full_like(e, KV4_MARK), e + 127), s, m, c
+
+
+def kv4_values(byte, s, m, c):
+    """The values [..., hd] in fp64 that quantised rows stand for."""
+    v = (m.double()[..., None] + s.double()[..., None] * c.double()).flatten(-2)
+    v = v * torch.pow(2.0, (byte.double() - 127))[..., None]
+    return torch.where((byte == KV4_MARK)[..., None], torch.full_like(v, math.nan), v)
+
+
+def kv4_places(hd, row):
+    """Where row `row` (0 .. 15) of a block keeps its parts: the 4-bit steps of K's and V's codes [hd] from the block's
+    start, and the bytes of K's s and m [hd / 32], V's s and m, K's and V's exponent."""
+    groups = hd // 32
+    k_code, v_code = [], []
+    for d in range(hd):
+        i, inside = d // 32, d % 32
+        t, b = inside // 8, inside % 8
+        word = (((i // 4) ^ (row & 1)) * 16 + 4 * t + i % 4) if hd == 256 else t * groups + i
+        k_code.append(2 * (row * hd // 2 + 4 * word) + b)
+        g, b = inside // 4, inside % 4
+        per = 256 // hd                                          # rows in 128 bytes
+        flip = {256: 2 * (row // 2 % 4), 128: 4 * (row // 2 % 4), 64: 8 * (row // 4 % 2)}[hd]
+        byte = 8 * hd + row // per * 128 + ((g + 8 * (row % per)) ^ flip) * (hd // 16) + 2 * i
+        v_code.append(2 * byte + b)
+    slot = 4 * (row % 8 // 2) + 2 * (row // 8) + row % 2
+    ks = [16 * hd + 2 * (row * groups + i) for i in range(groups)]
+    vs = [18 * hd + 2 * (16 * i + slot) for i in range(groups)]
+    at = {"k_s": ks, "k_m": [x + hd for x in ks], "v_s": vs, "v_m": [x + hd for x in vs]}
+    return k_code, v_code, at, 20 * hd + row, 20 * hd + 16 + row
+
+
+def kv4_put(block, row, k, v):
+    """Write rows k, v [hd] into row `row` of one block (a uint8 vector of 20 hd + 32 bytes), in place."""
+    hd = k.shape[-1]
+    k_code, v_code, at, ke, ve = kv4_places(hd, row)
+    for y, codes, name, e_at in ((k, k_code, "k", ke), (v, v_code, "v", ve)):
+        byte, s, m, c = kv4_quantise(y)
+        for place, code in zip(codes, c.flatten().tolist()):
+            old = int(block[place // 2])
+            block[place // 2] = (old & 0xF0) | int(code) if place % 2 == 0 else (old & 0x0F) | (int(code) << 4)
+        for part, x in (("s", s), ("m", m)):
+            raw = (x + 0.0).half().view(torch.uint8)
+            for j, place in enumerate(at[f"{name}_{part}"]):
+                block[place], block[place + 1] = raw[2 * j], raw[2 * j + 1]
+        block[e_at] = int(byte)
+
+
+def kv4_get(blocks, hd):
+    """K and V values [n, 16, hd] in fp64 of blocks [n, 20 hd + 32]."""
+    out = [[], []]
+    for row in range(16):
+        k_code, v_code, at, ke, ve = kv4_places(hd, row)
+        for which, (codes, name, e_at) in enumerate(((k_code, "k", ke), (v_code, "v", ve))):
+            place = torch.tensor(codes, device=blocks.device)
+            byte = blocks[:, place // 2].int()
+            c = torch.where(place % 2 == 0, byte & 15, byte >> 4).unflatten(-1, (-1, 32))
+            parts = [torch.stack((blocks[:, at[f"{name}_{p}"]], blocks[:, [x + 1 for x in at[f"{name}_{p}"]]]), -1)
+                     .contiguous().view(torch.half).squeeze(-1) for p in ("s", "m")]
+            out[which].append(kv4_values(blocks[:, e_at].int(), *parts, c))
+    return tuple(torch.stack(x, 1) for x in out)
+
+
+def kv4_head_row(x, w, norm_mode, eps, cos=None, sin=None):
+    """Head norm (-1 none, 0 plain, 1 zero-centred) and rotation of rows x [..., hd] as append computes them: rounded to
+    bf16 where the bf16 model rounds, the norm's sum and root in fp64; cos / sin [..., rot / 2]."""
+    def rounded(y):
+        return y.float().bfloat16().double()
+    x = x.double()
+    if norm_mode >= 0:
+        f = x * (1.0 / torch.sqrt(x.square().sum(-1, keepdim=True) / x.shape[-1] + eps))
+        x = rounded(rounded(f) * w.double()) if norm_mode == 0 else rounded(f * (1.0 + w.double()))
+    if cos is not None:
+        h = cos.shape[-1]
+        c, s = cos.double(), sin.double()
+        a, b = x[..., :h], x[..., h:2 * h]
+        x = torch.cat((rounded(rounded(a * c) + rounded(-b * s)), rounded(rounded(b * c) + rounded(a * s)),
+                       x[..., 2 * h:]), -1)
+    return x
