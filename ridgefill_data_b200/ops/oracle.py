@@ -309,8 +309,8 @@ def kv4_put(block, row, k, v):
         block[e_at] = int(byte)
 
 
-def kv4_get(blocks, hd):
-    """K and V values [n, 16, hd] in fp64 of blocks [n, 20 hd + 32]."""
+def kv4_get(blocks, hd, steps_only=False):
+    """K and V values [n, 16, hd] in fp64 of blocks [n, 20 hd + 32]; steps_only: their part 2^e s c above the minimum."""
     out = [[], []]
     for row in range(16):
         k_code, v_code, at, ke, ve = kv4_places(hd, row)
@@ -320,6 +320,8 @@ def kv4_get(blocks, hd):
             c = torch.where(place % 2 == 0, byte & 15, byte >> 4).unflatten(-1, (-1, 32))
             parts = [torch.stack((blocks[:, at[f"{name}_{p}"]], blocks[:, [x + 1 for x in at[f"{name}_{p}"]]]), -1)
                      .contiguous().view(torch.half).squeeze(-1) for p in ("s", "m")]
+            if steps_only:
+                parts[1] = torch.zeros_like(parts[1])
             out[which].append(kv4_values(blocks[:, e_at].int(), *parts, c))
     return tuple(torch.stack(x, 1) for x in out)
 

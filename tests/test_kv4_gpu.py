@@ -220,10 +220,14 @@ def _filled(lens, hkv, page, hd, seed=0, stale=True, vscale=1.0):
 
 
 def _reference(q, pool, pages, pos, scale, gate=None, gate_head=0):
-    """(out, error bound) [R, hq * hd] in fp64. The bound counts, per output of head h with P the softmax and
-    A = sum_j P_j |V_j|: the final rounding 2^-8 |out|; P and P s rounded to 11 bits (2 2^-11 A, an absolute 2^-24
-    where they are subnormal, of weights up to 2^14: below 2^-30 A n); the scores in 32-bit sums of exact products,
-    2^-18 sum_d |q_d K_jd| scale at most (hd terms of 2^-24 and the query sums' 2^-22), which moves A by twice that."""
+    """(out, error bound) [R, hq * hd] in fp64. A value is V = M + C, M = 2^e m its group's minimum and C = 2^e s c the
+    steps above it. Per output of head h, with P the softmax, the bound counts
+      the final rounding to bf16: 2^-8 |out|
+      P rounded to 11 bits, a factor of the whole value: 2^-11 sum_j P_j |V_j|
+      P s rounded to 11 bits, a factor of the steps alone: 2^-11 sum_j P_j C_j; both absolute where they fall below
+      2^-14: P is held so that the largest is between 2^6 and 2^14, so below 2^-30 of sum_j C_j over n keys
+      the scores, 32-bit sums of exact products over hd dims (2^-24 each) with the query's group sums held to 22 bits:
+      below 2^-18 of max_j sum_d |q_d| (|M_jd| + C_jd) scale, which moves the weighted mean by twice that."""
     hkv, hd, page = pool.shape[1], q.shape[2], pool.shape[2] * 16
     R, hq = q.shape[:2]
     G = hq // hkv
@@ -235,14 +239,15 @@ def _reference(q, pool, pages, pos, scale, gate=None, gate_head=0):
             continue
         blocks = pool[pages[s].long()[:-(-n // page)]].transpose(0, 1).reshape(-1, pool.shape[3])
         k, v = (t.view(hkv, -1, hd)[:, :n] for t in ops.kv4_get(blocks, hd))
+        kc, vc = (t.view(hkv, -1, hd)[:, :n] for t in ops.kv4_get(blocks, hd, steps_only=True))
         for h in range(hq):
             qq = q[s, h].double()
             x = (k[h // G] @ qq) * scale
             p = torch.softmax(x, 0)
             out[s, h] = p @ v[h // G]
-            spread = 2.0 ** -18 * (k[h // G].abs() @ qq.abs()).max() * abs(scale)
-            A = p @ v[h // G].abs()
-            bound[s, h] = 2.0 ** -8 * out[s, h].abs() + (2.0 ** -10 + 2 * spread + n * 2.0 ** -30) * A
+            spread = 2.0 ** -18 * (((k - kc).abs() + kc)[h // G] @ qq.abs()).max() * abs(scale)
+            A, C = p @ v[h // G].abs(), p @ vc[h // G]
+            bound[s, h] = (2.0 ** -8 * out[s, h].abs() + (2.0 ** -11 + 2 * spread) * A + (2.0 ** -11 + n * 2.0 ** -30) * C)
     if gate is not None:
         sg = torch.sigmoid(torch.stack([gate[:, h * gate_head:h * gate_head + hd] for h in range(hq)], 1).double())
         out, bound = out * sg, bound * sg + 2.0 ** -18 * (out * sg).abs()
