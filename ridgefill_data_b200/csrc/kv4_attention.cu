@@ -31,7 +31,8 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 4;
 constexpr float kLow = -1e30f;   // below every score: exp2 of a difference to it is 0, never NaN
 
-__host__ __device__ constexpr int split_keys(int p) { return 256 * (p / (256 * kKv4Splits) + 1); }
+constexpr int kUnit = 512;       // keys of a split, up to kKv4Splits of them; then a multiple
+__host__ __device__ constexpr int split_keys(int p) { return kUnit * (p / (kUnit * kKv4Splits) + 1); }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -46,6 +47,15 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// the same with a zero accumulator
+__device__ __forceinline__ void mma_f16_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
@@ -86,66 +96,133 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t* w) {
   }
 }
 
+// The next kernel of the stream may start before this one ends (its first act is to wait for it) / that wait.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// out = o / sum * sigmoid(gate) for 4 dims of a head. A sum of -inf (or NaN) tells of a visible row with non-finite
+// values; 0 of no row at all.
+__device__ __forceinline__ void finish(const Kv4AttnArgs& a, int r, int col, int h, int e, float4 o, float sum) {
+  const float n = sum == 0.f ? 0.f : sum > 0.f && sum < INFINITY ? 1.f / sum : __int_as_float(0x7fffffff);
+  float g[4] = {n, n, n, n};
+  if (a.gate != nullptr) {
+    float z[4];
+    kv4_load<4>(a.gate + (long)r * a.gate_row + (long)h * a.gate_head + e, z);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = n / (1.f + __expf(-z[j]));
+  }
+  const float v[4] = {o.x * g[0], o.y * g[1], o.z * g[2], o.w * g[3]};
+  kv4_store<4>(a.out + (long)r * a.out_row + col, v);
+}
+
 constexpr float kTop = 14.f;    // P <= 2^14
 constexpr float kRoom = 6.f;    // a raised maximum leaves P <= 2^6
+
+// The query heads of one KV head as B fragments, shared by the CTA's warps.
+template <int HD>
+struct Query {
+  uint2 q[HD / 32][2][32];   // group, half (of 8 dims of a lane: even and odd nibbles), lane
+  uint2 sums[32];            // group sums: high and low halves
+  float scale[8];            // per column: scale log2(e) 2^e_q
+  unsigned top[kWarps][8];
+  float part[HD / 32][8];    // sums by group and column
+};
+
+// query rows [G, HD] of one KV head, as fp16 q 2^-e_q with max |q| 2^-e_q in [2^9, 2^10); all warps, each its groups
+template <int HD>
+__device__ __forceinline__ void load_query(Query<HD>& s, const Kv4AttnArgs& a, const __nv_bfloat16* rows, int G, int warp,
+                                           int lane) {
+  constexpr int NG = HD / 32, MINE = (NG + kWarps - 1) / kWarps;
+  const int g = lane >> 2, t = lane & 3;
+  uint4 raw[MINE];
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < MINE; ++j) {
+    const int i = warp + kWarps * j;
+    raw[j] = make_uint4(0u, 0u, 0u, 0u);
+    if (g < G && i < NG) raw[j] = *reinterpret_cast<const uint4*>(rows + (long)g * a.q_head + 32 * i + 8 * t);
+    const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) top = __vmaxu2(top, w[x] & 0x7fff7fffu);
+  }
+  top = max(top & 0xffffu, top >> 16);
+  top = max(top, __shfl_xor_sync(kFull, top, 1));
+  top = max(top, __shfl_xor_sync(kFull, top, 2));
+  if (t == 0) s.top[warp][g] = top;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kWarps; ++j) top = max(top, s.top[j][g]);
+  const bool bad = top >= 0x7f80u;
+  const int e = min(max((int)(top >> 7) - 127, -100), 127) - 9;   // at 2^-100 and below fewer bits are kept
+  const float down = bad ? 0.f : kv4_pow2(-e);
+#pragma unroll
+  for (int j = 0; j < MINE; ++j) {
+    const int i = warp + kWarps * j;
+    if (i >= NG) break;
+    const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+    float v[8], sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      // a row with a non-finite value: zeros (its scale is NaN)
+      v[2 * x] = bad ? 0.f : bf16_lo(w[x]) * down;
+      v[2 * x + 1] = bad ? 0.f : bf16_hi(w[x]) * down;
+      sum += v[2 * x] + v[2 * x + 1];
+    }
+    sum += __shfl_xor_sync(kFull, sum, 1);
+    sum += __shfl_xor_sync(kFull, sum, 2);
+    if (t == 0) s.part[i][g] = sum;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      s.q[i][h][lane] = make_uint2(pack_half(v[2 * h], v[2 * h + 4]),
+                                   pack_half(v[2 * h + 1] * 0.0625f, v[2 * h + 5] * 0.0625f));
+  }
+  if (warp == 0 && t == 0) s.scale[g] = bad ? __int_as_float(0x7fffffff) : ldexpf(a.scale_log2, e);
+  __syncthreads();
+  if (warp == 0) {
+    float a0 = 0.f, a1 = 0.f;
+    if (2 * t < NG) a0 = s.part[2 * t][g], a1 = s.part[2 * t + 1][g];
+    const uint32_t hi = pack_half(a0, a1);
+    const float2 f = unpack_half(hi);
+    s.sums[lane] = make_uint2(hi, pack_half(a0 - f.x, a1 - f.y));
+  }
+  __syncthreads();
+}
 
 template <int HD>
 struct Warp {
   using L = Kv4L<HD>;
   static constexpr int NG = L::NG;
-  uint32_t q[NG][2][2];    // B fragments of the query heads: group, half (even, odd nibbles' dims), register
-  uint32_t qs[2];          // their group sums: high and low halves
-  float cs[2];             // per column 2t, 2t + 1: scale log2(e) 2^e_q
+  static constexpr bool kHold = HD != 256;   // the fragments in registers, or read from shared memory at each use
+  uint2 held[kHold ? NG : 1][2];
+  const Query<HD>* query;
+  int lane_;
+  uint2 qs;                // group sums
+  float cs[2];             // per column 2t, 2t + 1
   float o[NG][2][4];       // output accumulators: group, tile
   float om[4];             // sums of m P
   float ref[2], l[2];
 
-  // query rows [G, HD] of one KV head, as fp16 q 2^-e_q with max |q| 2^-e_q in [2^9, 2^10)
-  __device__ __forceinline__ void load_q(const Kv4AttnArgs& a, const __nv_bfloat16* rows, int G, int lane) {
-    const int g = lane >> 2, t = lane & 3;
-    float v[NG][8];
-    unsigned top = 0;
+  __device__ __forceinline__ uint2 q(int i, int h) const {
+    if constexpr (kHold) return held[i][h];
+    return query->q[i][h][lane_];
+  }
+
+  __device__ __forceinline__ void start(const Query<HD>& s, int lane) {
+    query = &s;
+    lane_ = lane;
+    if constexpr (kHold) {
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
+      for (int i = 0; i < NG; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      if (g < G) kv4_load<8>(rows + (long)g * a.q_head + 32 * i + 8 * t, v[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+        for (int h = 0; h < 2; ++h) held[i][h] = s.q[i][h][lane];
     }
-    top = max(top, __shfl_xor_sync(kFull, top, 1));
-    top = max(top, __shfl_xor_sync(kFull, top, 2));
-    const bool bad = top >= 0x7f800000u;
-    const int e = min(max((int)(top >> 23) - 127, -100), 127) - 9;   // q 2^-e; 2^-100 and below keep fewer bits
-    const float down = kv4_pow2(-e / 2), down2 = kv4_pow2(-e - -e / 2);
-    float sum[NG];
+    qs = s.sums[lane];
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      sum[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[i][j] = bad ? 0.f : v[i][j] * down * down2;
-        sum[i] += v[i][j];
-      }
-      sum[i] += __shfl_xor_sync(kFull, sum[i], 1);
-      sum[i] += __shfl_xor_sync(kFull, sum[i], 2);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        q[i][h][0] = pack_half(v[i][2 * h], v[i][2 * h + 4]);
-        q[i][h][1] = pack_half(v[i][2 * h + 1] * 0.0625f, v[i][2 * h + 5] * 0.0625f);
-      }
+    for (int c = 0; c < 2; ++c) {
+      cs[c] = s.scale[2 * (lane & 3) + c];
+      ref[c] = kLow;
+      l[c] = 0.f;
     }
-    float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-    for (int i = 0; i < NG; i += 2)
-      if (i == 2 * t) a0 = sum[i], a1 = sum[i + 1];
-    qs[0] = pack_half(a0, a1);
-    const float2 hi = unpack_half(qs[0]);
-    qs[1] = pack_half(a0 - hi.x, a1 - hi.y);
-    // the scale of column g sits in lanes 4 g ..; columns 2t, 2t + 1 belong to this lane's scores
-    const float c = bad ? __int_as_float(0x7fffffff) : ldexpf(a.scale_log2, e);
-    cs[0] = __shfl_sync(kFull, c, 8 * t);
-    cs[1] = __shfl_sync(kFull, c, 8 * t + 4);
 #pragma unroll
     for (int i = 0; i < NG; ++i)
 #pragma unroll
@@ -154,64 +231,71 @@ struct Warp {
         for (int j = 0; j < 4; ++j) o[i][x][j] = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) om[j] = 0.f;
-    ref[0] = ref[1] = kLow;
-    l[0] = l[1] = 0.f;
   }
 
-  // one block of 16 keys; LAST: only its first `live` rows exist (the others' bytes may be anything)
-  template <bool LAST>
-  __device__ __forceinline__ void block(const uint8_t* b, int live, int lane) {
+  // NB blocks of 16 keys at b; LAST: only the first live[u] rows of block u exist (the others' bytes may be anything)
+  template <bool LAST, int NB>
+  __device__ __forceinline__ void blocks(const uint8_t* b, const int (&live)[NB], int lane) {
     const int g = lane >> 2, t = lane & 3;
-    // scores: rows g and g + 8, columns 2t and 2t + 1
+    // scores: rows g and g + 8, columns 2t and 2t + 1; y = score + size of the V row (its byte)
     constexpr int KW = NG < 4 ? NG : 4;    // words of one load
-    float s[4] = {0.f, 0.f, 0.f, 0.f}, cm[4] = {0.f, 0.f, 0.f, 0.f};
-    {
+    float y[NB][4], iv[NB][2];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const uint8_t* k = b + u * L::BYTES;
+      float s[4], cm[4];
       uint32_t ks[2][NG / 2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) lds<NG / 2>(b + L::KS + (g + 8 * r) * NG * 2, ks[r]);
+      for (int r = 0; r < 2; ++r) lds<NG / 2>(k + L::KS + (g + 8 * r) * NG * 2, ks[r]);
 #pragma unroll
       for (int i0 = 0; i0 < NG; i0 += KW) {
         uint32_t w[2][KW];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) lds<KW>(b + L::k_word(g + 8 * r, t, i0), w[r]);
+        for (int r = 0; r < 2; ++r) lds<KW>(k + L::k_word(g + 8 * r, t, i0), w[r]);
 #pragma unroll
         for (int i = i0; i < i0 + KW; ++i) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t x = w[0][i - i0], y = w[1][i - i0];
-          mma_f16(acc, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, q[i][0][0], q[i][0][1]);
-          x >>= 8, y >>= 8;
-          mma_f16(acc, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, q[i][1][0], q[i][1][1]);
+          float acc[4];
+          uint32_t x = w[0][i - i0], z = w[1][i - i0];
+          const uint2 q0 = q(i, 0), q1 = q(i, 1);
+          mma_f16_new(acc, x & 0x000f000fu, z & 0x000f000fu, x & 0x00f000f0u, z & 0x00f000f0u, q0.x, q0.y);
+          x >>= 8, z >>= 8;
+          mma_f16(acc, x & 0x000f000fu, z & 0x000f000fu, x & 0x00f000f0u, z & 0x00f000f0u, q1.x, q1.y);
           const float2 p0 = unpack_half(ks[0][i / 2]), p1 = unpack_half(ks[1][i / 2]);
           const float s0 = i & 1 ? p0.y : p0.x, s1 = i & 1 ? p1.y : p1.x;
-          s[0] = fmaf(s0, acc[0], s[0]);
-          s[1] = fmaf(s0, acc[1], s[1]);
-          s[2] = fmaf(s1, acc[2], s[2]);
-          s[3] = fmaf(s1, acc[3], s[3]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[j] = i == 0 ? (j < 2 ? s0 : s1) * acc[j] : fmaf(j < 2 ? s0 : s1, acc[j], s[j]);
         }
       }
       uint32_t m0 = 0, m1 = 0;
       if (2 * t < NG) {
-        m0 = *reinterpret_cast<const uint32_t*>(b + L::KM + g * NG * 2 + 4 * t);
-        m1 = *reinterpret_cast<const uint32_t*>(b + L::KM + (g + 8) * NG * 2 + 4 * t);
+        m0 = *reinterpret_cast<const uint32_t*>(k + L::KM + g * NG * 2 + 4 * t);
+        m1 = *reinterpret_cast<const uint32_t*>(k + L::KM + (g + 8) * NG * 2 + 4 * t);
       }
-      mma_f16(cm, m0, m1, m0, m1, qs[0], qs[1]);
-    }
-    const int ve0 = b[L::VE + g], ve1 = b[L::VE + g + 8];
-    const float kz0 = kv4_size(b[L::KE + g]), kz1 = kv4_size(b[L::KE + g + 8]);
-    const float nan = __int_as_float(0x7fffffff);
-    const float e0 = ve0 == kKv4Mark ? nan : (float)(ve0 - 127), e1 = ve1 == kKv4Mark ? nan : (float)(ve1 - 127);
-    float y[4];
+      mma_f16_new(cm, m0, m1, m0, m1, qs.x, qs.y);
+      // sizes by their bytes: a marked row's 255 makes the K size infinite (its score 0 x inf = NaN) and the V size's
+      // inverse -inf, which the sum keeps (or turns to NaN) and the join answers with NaN
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x = fmaf(s[j], 16777216.f, cm[j]) * ((j < 2 ? kz0 : kz1) * cs[j & 1]);
-      y[j] = x + (j < 2 ? e0 : e1);
-      if (LAST && g + (j < 2 ? 0 : 8) >= live) y[j] = -INFINITY;
+      for (int r = 0; r < 2; ++r) {
+        const int ve = k[L::VE + g + 8 * r];
+        const float kz = __int_as_float(k[L::KE + g + 8 * r] << 23), e = (float)ve;
+        iv[u][r] = __int_as_float((254 - ve) << 23);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          y[u][2 * r + c] = fmaf(fmaf(s[2 * r + c], 16777216.f, cm[2 * r + c]), kz * cs[c], e);
+        if (LAST && g + 8 * r >= live[u]) y[u][2 * r] = y[u][2 * r + 1] = -INFINITY, iv[u][r] = 0.f;
+      }
     }
-    const bool over = fmaxf(y[0], y[2]) > ref[0] + kTop || fmaxf(y[1], y[3]) > ref[1] + kTop;
-    if (__any_sync(kFull, over)) {
+    float top[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      top[c] = fmaxf(y[0][c], y[0][c + 2]);
+#pragma unroll
+      for (int u = 1; u < NB; ++u) top[c] = fmaxf(top[c], fmaxf(y[u][c], y[u][c + 2]));
+    }
+    if (__any_sync(kFull, top[0] > ref[0] + kTop || top[1] > ref[1] + kTop)) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float m = fmaxf(y[c], y[c + 2]);
+        float m = top[c];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
         m = fmaxf(ref[c], m - kRoom);
@@ -225,39 +309,47 @@ struct Warp {
         om[c] *= f, om[c + 2] *= f;
       }
     }
-    float p[4];
+    uint32_t pb[NB][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = ex2(y[j] - ref[j & 1]);
-    const float iv0 = __int_as_float((254 - min(ve0, 253)) << 23), iv1 = __int_as_float((254 - min(ve1, 253)) << 23);
-    l[0] = fmaf(p[0], iv0, fmaf(p[2], iv1, l[0]));
-    l[1] = fmaf(p[1], iv0, fmaf(p[3], iv1, l[1]));
-    const uint32_t b0 = transpose_8x8(pack_half(p[0], p[1])), b1 = transpose_8x8(pack_half(p[2], p[3]));
+    for (int u = 0; u < NB; ++u) {
+      float p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[j] = ex2(y[u][j] - ref[j & 1]);
+        l[j & 1] = fmaf(p[j], iv[u][j >> 1], l[j & 1]);
+      }
+      pb[u][0] = transpose_8x8(pack_half(p[0], p[1]));
+      pb[u][1] = transpose_8x8(pack_half(p[2], p[3]));
+    }
     // values: keys 2t, 2t + 1, 2t + 8, 2t + 9; tile x of group i: dims 32 i + 4 g + 2 x (rows g), + 1 (rows g + 8)
-    uint32_t keep0 = kFull, keep1 = kFull;
-    if constexpr (LAST) {
-      keep0 = (2 * t < live ? 0xffffu : 0u) | (2 * t + 1 < live ? 0xffff0000u : 0u);
-      keep1 = (2 * t + 8 < live ? 0xffffu : 0u) | (2 * t + 9 < live ? 0xffff0000u : 0u);
-    }
-    {
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const uint8_t* v = b + u * L::BYTES;
+      uint32_t keep[2] = {kFull, kFull};
+      if constexpr (LAST) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          keep[r] = (2 * t + 8 * r < live[u] ? 0xffffu : 0u) | (2 * t + 8 * r + 1 < live[u] ? 0xffff0000u : 0u);
+      }
       uint32_t m[2] = {0u, 0u};
-      if (g < NG) lds<2>(b + L::VM + g * 32 + 8 * t, m);
-      if constexpr (LAST) m[0] &= keep0, m[1] &= keep1;
-      mma_f16(om, m[0], 0u, m[1], 0u, b0, b1);
-    }
-    uint32_t w[4][NG / 2];
+      if (g < NG) lds<2>(v + L::VM + g * 32 + 8 * t, m);
+      if constexpr (LAST) m[0] &= keep[0], m[1] &= keep[1];
+      mma_f16(om, m[0], 0u, m[1], 0u, pb[u][0], pb[u][1]);
+      uint32_t w[4][NG / 2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) lds<NG / 2>(b + L::v_chunk(2 * t + (j & 1) + 8 * (j >> 1), g), w[j]);
+      for (int j = 0; j < 4; ++j) lds<NG / 2>(v + L::v_chunk(2 * t + (j & 1) + 8 * (j >> 1), g), w[j]);
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      uint32_t sc[2];
-      lds<2>(b + L::VS + i * 32 + 8 * t, sc);
-      if constexpr (LAST) sc[0] &= keep0, sc[1] &= keep1;
-      const uint32_t c0 = mul_half2(b0, sc[0]), c1 = mul_half2(b1, sc[1]);
-      const unsigned pick = i & 1 ? 0x7632 : 0x5410;
-      uint32_t x = __byte_perm(w[0][i / 2], w[1][i / 2], pick), z = __byte_perm(w[2][i / 2], w[3][i / 2], pick);
-      mma_f16(o[i][0], x & 0x000f000fu, x & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, c0, c1);
-      x >>= 8, z >>= 8;
-      mma_f16(o[i][1], x & 0x000f000fu, x & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, c0, c1);
+      for (int i = 0; i < NG; ++i) {
+        uint32_t sc[2];
+        lds<2>(v + L::VS + i * 32 + 8 * t, sc);
+        if constexpr (LAST) sc[0] &= keep[0], sc[1] &= keep[1];
+        const uint32_t c0 = mul_half2(pb[u][0], sc[0]), c1 = mul_half2(pb[u][1], sc[1]);
+        const unsigned pick = i & 1 ? 0x7632 : 0x5410;
+        uint32_t x = __byte_perm(w[0][i / 2], w[1][i / 2], pick), z = __byte_perm(w[2][i / 2], w[3][i / 2], pick);
+        mma_f16(o[i][0], x & 0x000f000fu, x & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, c0, c1);
+        x >>= 8, z >>= 8;
+        mma_f16(o[i][1], x & 0x000f000fu, x & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, c0, c1);
+      }
     }
   }
 
@@ -287,84 +379,104 @@ struct Warp {
 
 template <int HD>
 struct Cfg {
-  static constexpr int STAGES = HD == 256 ? 3 : 4;
-  static constexpr int RING = kWarps * STAGES * Kv4L<HD>::BYTES;
+  static constexpr int NB = HD == 256 ? 1 : 2;          // blocks of a stage
+  static constexpr int STAGES = HD == 256 ? 3 : 2;
+  static constexpr int CTAS = HD == 256 ? 3 : HD == 128 ? 4 : 6;   // on an SM: its registers bound the compiler's
+  static constexpr int RING = kWarps * STAGES * NB * Kv4L<HD>::BYTES;
   static constexpr int JOIN = kWarps * 8 * HD * 4;     // the warps' outputs, in the ring's place after the last block
   static constexpr int SMEM = RING > JOIN ? RING : JOIN;
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kWarps * 32) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a, int r0) {
+__global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
+    kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a, int r0) {
   using L = Kv4L<HD>;
-  constexpr int ST = Cfg<HD>::STAGES;
+  constexpr int ST = Cfg<HD>::STAGES, NB = Cfg<HD>::NB;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kWarps][ST];
   __shared__ float refs[kWarps][8], ls[kWarps][8];
+  __shared__ Query<HD> query;
   const int s = blockIdx.x, g = blockIdx.y, sq = blockIdx.z, r = r0 + sq;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.hq / a.c.hkv;
+  allow_next();
   const int p = a.pos[r];
-  if (p >= a.c.rows[sq]) {
-    if (s == 0 && g == 0 && threadIdx.x == 0) record_error(a.err, kErrBadIndex);
+  if (p < 0 || p >= a.c.rows[sq]) {
+    if (p >= 0 && s == 0 && g == 0 && threadIdx.x == 0) record_error(a.err, kErrBadIndex);
+    if (s == 0)
+      for (int x = threadIdx.x; x < G * HD / 4; x += kWarps * 32)
+        kv4_store<4>(a.out + (long)r * a.out_row + g * G * HD + 4 * x, {0.f, 0.f, 0.f, 0.f});
     return;
   }
-  if (p < 0) return;
   const int keys = split_keys(p), start = s * keys;
   if (start > p) return;
   const int end = min(start + keys, p + 1);
-  // blocks warp, warp + 4, ... of the split; lane x of the first ST drives stage x: its barrier, its copies, the page
-  // id of the copy after next
+  // the split's blocks in runs of NB: runs warp, warp + 4, ... Lane x of the first ST NB drives slot x of the ring: its
+  // copies, half of its stage's barrier, and the page id of the copy after next
   const int blocks = (end - start + 15) / 16;
-  uint8_t* ring = smem + warp * ST * L::BYTES;
+  uint8_t* ring = smem + warp * ST * NB * L::BYTES;
   uint64_t* bar = bars[warp];
-  int mine = warp + kWarps * lane;                 // the block this lane loads next
-  int page = 0;                                    // its page
-  bool good = false;
+  int mine = NB * (warp + kWarps * (lane / NB)) + lane % NB;   // the block this lane loads next: block `in` of page
+  const int per = a.c.page_size / 16;                          // `page`, whose id is fetched one turn ahead
+  const int first = start / 16 + mine;
+  int page = first / per, in = first % per, id = -1;
+  const int step = NB * kWarps * ST / per, left = NB * kWarps * ST % per;
   const int* table = a.c.pages[sq];
+  const long head = (long)g * per;
+  bool good = false;
   auto issue = [&]() {
-    const int row = start + 16 * mine;
-    good = page >= 0 && page < a.c.num_pages;
-    if (good) {
-      const long slab = ((long)page * a.c.hkv + g) * (a.c.page_size / 16) + (row % a.c.page_size) / 16;
-      mbar_expect_tx(bar + lane, L::BYTES);
-      bulk_load(ring + lane * L::BYTES, a.c.pool + slab * L::BYTES, L::BYTES, bar + lane);
-    } else {
+    uint64_t* full = bar + lane / NB;
+    good = mine < blocks;
+    if (good && (id < 0 || id >= a.c.num_pages)) {
       record_error(a.err, kErrBadIndex);
-      mbar_arrive(bar + lane);
+      good = false;
     }
-    mine += kWarps * ST;
-    if (mine < blocks) page = __ldg(table + (start + 16 * mine) / a.c.page_size);
+    if (good) {
+      mbar_expect_tx(full, L::BYTES);
+      bulk_load(ring + lane * L::BYTES, a.c.pool + ((long)id * a.c.hkv * per + head + in) * L::BYTES, L::BYTES, full);
+    } else {
+      mbar_arrive(full);
+    }
+    mine += NB * kWarps * ST;
+    page += step, in += left;
+    if (in >= per) in -= per, ++page;
+    if (mine < blocks) id = __ldg(table + page);
   };
-  if (lane < ST) {
-    mbar_init(bar + lane, 1);
-    fence_barrier_init();
-    if (mine < blocks) {
-      page = __ldg(table + (start + 16 * mine) / a.c.page_size);
-      issue();
-    }
+  if (lane < ST) mbar_init(bar + lane, NB);
+  fence_barrier_init();
+  __syncwarp();
+  if (lane < ST * NB && mine - lane % NB < blocks) {
+    if (mine < blocks) id = __ldg(table + page);
+    issue();
   }
   __syncwarp();
+  load_query<HD>(query, a, a.q + (long)r * a.q_row + (long)g * G * a.q_head, G, warp, lane);
   Warp<HD> w;
-  w.load_q(a, a.q + (long)r * a.q_row + (long)g * G * a.q_head, G, lane);
+  w.start(query, lane);
   int stage = 0, phase = 0;
-  for (int k = warp; k < blocks; k += kWarps) {
+  for (int k = NB * warp; k < blocks; k += NB * kWarps) {
     if (!__all_sync(kFull, mbar_wait(bar + stage, phase, a.err, kErrTimeoutProducer))) {
-      for (int j = 0; j < ST && k < blocks; ++j, k += kWarps) {   // no copy may outlive the CTA
+      for (int j = 0; j < ST && k < blocks; ++j, k += NB * kWarps) {   // no copy may outlive the CTA
         mbar_wait(bar + stage, phase, a.err, kErrTimeoutDrain);
         if (++stage == ST) stage = 0, phase ^= 1;
       }
       break;
     }
-    const uint8_t* b = ring + stage * L::BYTES;
-    if (__shfl_sync(kFull, good, stage)) {
-      const int live = end - start - 16 * k;
-      if (live >= 16)
-        w.template block<false>(b, 16, lane);
-      else
-        w.template block<true>(b, live, lane);
+    const uint8_t* b = ring + stage * NB * L::BYTES;
+    const unsigned loaded = __ballot_sync(kFull, good) >> (stage * NB);
+    int live[NB];
+    bool full = true;
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      live[u] = loaded >> u & 1 ? end - start - 16 * (k + u) : 0;
+      full = full && live[u] >= 16;
     }
+    if (full)
+      w.template blocks<false, NB>(b, live, lane);
+    else
+      w.template blocks<true, NB>(b, live, lane);
     __syncwarp();
-    if (lane == stage && mine < blocks) issue();
+    if (lane / NB == stage && mine - lane % NB < blocks) issue();
     if (++stage == ST) stage = 0, phase ^= 1;
   }
   __syncthreads();                                 // every copy has landed: the ring's memory is free
@@ -372,45 +484,90 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attn_kernel(const __grid_cons
   w.store(refs[warp], ls[warp], outs + warp * 8 * HD, G, lane);
   __syncthreads();
   const long base = (((long)r * a.c.hkv + g) * a.splits + s) * G;
-  for (int x = threadIdx.x; x < G * HD; x += kWarps * 32) {
-    const int h = x / HD;
-    float M = refs[0][h], S = 0.f, O = 0.f;
+  const bool only = p < keys;                      // one split holds every row: its join is the output
+  if (threadIdx.x < G) {                           // the warps' weights in place of their references
+    const int h = threadIdx.x;
+    float M = refs[0][h], S = 0.f;
 #pragma unroll
     for (int i = 1; i < kWarps; ++i) M = fmaxf(M, refs[i][h]);
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-      const float f = exp2f(refs[i][h] - M);
+      const float f = ex2(refs[i][h] - M);
       S = fmaf(ls[i][h], f, S);
-      O = fmaf(outs[i * 8 * HD + x], f, O);
+      refs[i][h] = f;
     }
-    a.part_o[base * HD + x] = O;
-    if (x % HD == 0) a.part_ml[(base + h) * 2] = M, a.part_ml[(base + h) * 2 + 1] = S;
+    ls[0][h] = S;
+    if (!only) *reinterpret_cast<float2*>(a.part_ml + (base + h) * 2) = make_float2(M, S);
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < G * HD / 4; x += kWarps * 32) {
+    const int h = x / (HD / 4);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const float f = refs[i][h];
+      const float4 v = reinterpret_cast<const float4*>(outs + i * 8 * HD)[x];
+      sum.x = fmaf(v.x, f, sum.x), sum.y = fmaf(v.y, f, sum.y);
+      sum.z = fmaf(v.z, f, sum.z), sum.w = fmaf(v.w, f, sum.w);
+    }
+    if (only)
+      finish(a, r, (g * G) * HD + 4 * x, g * G + h, 4 * x - h * HD, sum, ls[0][h]);
+    else
+      reinterpret_cast<float4*>(a.part_o + base * HD)[x] = sum;
   }
 }
 
-__global__ void kv4_combine_kernel(Kv4AttnArgs a, int r0) {
-  const int HD = blockDim.x, G = a.hq / a.c.hkv;
-  const int h = blockIdx.x, sq = blockIdx.y, r = r0 + sq, e = threadIdx.x;
+constexpr int kJoin = 8;    // split lanes of the combine: thread (x, y) sums float4 x of splits y, y + kJoin, ...
+
+template <int HD>
+__global__ void __launch_bounds__(HD / 4 * kJoin) kv4_combine_kernel(const __grid_constant__ Kv4AttnArgs a, int r0) {
+  __shared__ float f[kKv4Splits];
+  __shared__ float4 part[kJoin][HD / 4];
+  const int G = a.hq / a.c.hkv;
+  const int h = blockIdx.x, sq = blockIdx.y, r = r0 + sq;
+  const int x = threadIdx.x % (HD / 4), y = threadIdx.x / (HD / 4);
+  wait_previous();
   const int p = a.pos[r];
-  float o = 0.f;
-  if (p >= 0 && p < a.c.rows[sq]) {
-    const int ns = p / split_keys(p) + 1;
-    const long base = ((long)r * a.c.hkv + h / G) * a.splits * G + h % G;
-    float M = kLow, S = 0.f;
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, a.part_ml[(base + (long)s * G) * 2]);
-    for (int s = 0; s < ns; ++s) {
-      const long i = base + (long)s * G;
-      const float f = exp2f(a.part_ml[i * 2] - M);
-      S = fmaf(a.part_ml[i * 2 + 1], f, S);
-      o = fmaf(a.part_o[i * HD + e], f, o);
-    }
-    o = S == 0.f ? 0.f : o / S;
-    if (a.gate != nullptr) {
-      const float z = __bfloat162float(a.gate[(long)r * a.gate_row + (long)h * a.gate_head + e]);
-      o *= 1.f / (1.f + __expf(-z));
-    }
+  if (p >= a.c.rows[sq] || p < split_keys(0)) return;   // no row, or one split: written by it
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float S = 0.f;
+  const int ns = p / split_keys(p) + 1;
+  const long base = ((long)r * a.c.hkv + h / G) * a.splits * G + h % G;
+  // every warp finds the largest maximum and the sum; the split's weight for all from the first
+  const int lane = threadIdx.x & 31;
+  float m[kKv4Splits / 32], l[kKv4Splits / 32], M = kLow;
+#pragma unroll
+  for (int j = 0; j < kKv4Splits / 32; ++j) {
+    const int s = lane + 32 * j;
+    const float2 ml = s < ns ? *reinterpret_cast<const float2*>(a.part_ml + (base + (long)s * G) * 2) : make_float2(kLow, 0.f);
+    m[j] = ml.x, l[j] = ml.y;
+    M = fmaxf(M, m[j]);
   }
-  a.out[(long)r * a.out_row + (long)h * HD + e] = __float2bfloat16(o);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, d));
+#pragma unroll
+  for (int j = 0; j < kKv4Splits / 32; ++j) {
+    const float w = exp2f(m[j] - M);
+    S = fmaf(l[j], w, S);
+    if (threadIdx.x < 32) f[lane + 32 * j] = w;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(kFull, S, d);
+  __syncthreads();
+#pragma unroll 4
+  for (int s = y; s < ns; s += kJoin) {
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + (base + (long)s * G) * HD + 4 * x);
+    o.x = fmaf(v.x, f[s], o.x), o.y = fmaf(v.y, f[s], o.y), o.z = fmaf(v.z, f[s], o.z), o.w = fmaf(v.w, f[s], o.w);
+  }
+  part[y][x] = o;
+  __syncthreads();
+  if (y > 0) return;
+#pragma unroll
+  for (int j = 1; j < kJoin; ++j) {
+    const float4 v = part[j][x];
+    o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+  }
+  finish(a, r, h * HD + 4 * x, h, 4 * x, o, S);
 }
 
 template <int HD>
@@ -423,13 +580,25 @@ void launch(const Kv4AttnArgs& a, int r0, int seqs, cudaStream_t stream) {
   });
   kv4_attn_kernel<HD><<<dim3(a.splits, a.c.hkv, seqs), kWarps * 32, Cfg<HD>::SMEM, stream>>>(a, r0);
   count_launch();
-  kv4_combine_kernel<<<dim3(a.hq, seqs), HD, 0, stream>>>(a, r0);
-  count_launch();
+  if (a.splits > 1) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.hq, seqs);
+    cfg.blockDim = dim3(HD / 4 * kJoin);
+    cfg.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kv4_combine_kernel<HD>, a, r0) != cudaSuccess)
+      throw std::runtime_error("kv4_attention: launch of the join failed");
+    count_launch();
+  }
 }
 
 }  // namespace
 
-int kv4_splits(int rows) { return rows <= 0 ? 1 : std::min(kKv4Splits, (rows - 1) / 256 + 1); }
+int kv4_splits(int rows) { return rows <= 0 ? 1 : std::min(kKv4Splits, (rows - 1) / kUnit + 1); }
 
 void kv4_attention(const Kv4AttnArgs& a, int r0, int seqs, cudaStream_t stream) {
   if (seqs <= 0) return;
