@@ -122,71 +122,77 @@ constexpr float kRoom = 6.f;    // a raised maximum leaves P <= 2^6
 template <int HD>
 struct Query {
   uint2 q[HD / 32][2][32];   // group, half (of 8 dims of a lane: even and odd nibbles), lane
-  uint2 sums[32];            // group sums: high and low halves
   float scale[8];            // per column: scale log2(e) 2^e_q
   unsigned top[kWarps][8];
-  float part[HD / 32][8];    // sums by group and column
+  float part[HD / 32][8];    // group sums by column
 };
 
-// query rows [G, HD] of one KV head, as fp16 q 2^-e_q with max |q| 2^-e_q in [2^9, 2^10); all warps, each its groups
+// The query heads [G, HD] of one KV head as fp16 q 2^-e_q with max |q| 2^-e_q in [2^9, 2^10). All warps, each the groups
+// it has loaded.
 template <int HD>
-__device__ __forceinline__ void load_query(Query<HD>& s, const Kv4AttnArgs& a, const __nv_bfloat16* rows, int G, int warp,
-                                           int lane) {
-  constexpr int NG = HD / 32, MINE = (NG + kWarps - 1) / kWarps;
-  const int g = lane >> 2, t = lane & 3;
+struct QueryLoad {
+  static constexpr int NG = HD / 32, MINE = (NG + kWarps - 1) / kWarps;
   uint4 raw[MINE];
-  unsigned top = 0;
+
+  __device__ __forceinline__ void load(const Kv4AttnArgs& a, const __nv_bfloat16* rows, int G, int warp, int lane) {
+    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int j = 0; j < MINE; ++j) {
-    const int i = warp + kWarps * j;
-    raw[j] = make_uint4(0u, 0u, 0u, 0u);
-    if (g < G && i < NG) raw[j] = *reinterpret_cast<const uint4*>(rows + (long)g * a.q_head + 32 * i + 8 * t);
-    const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-#pragma unroll
-    for (int x = 0; x < 4; ++x) top = __vmaxu2(top, w[x] & 0x7fff7fffu);
-  }
-  top = max(top & 0xffffu, top >> 16);
-  top = max(top, __shfl_xor_sync(kFull, top, 1));
-  top = max(top, __shfl_xor_sync(kFull, top, 2));
-  if (t == 0) s.top[warp][g] = top;
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kWarps; ++j) top = max(top, s.top[j][g]);
-  const bool bad = top >= 0x7f80u;
-  const int e = min(max((int)(top >> 7) - 127, -100), 127) - 9;   // at 2^-100 and below fewer bits are kept
-  const float down = bad ? 0.f : kv4_pow2(-e);
-#pragma unroll
-  for (int j = 0; j < MINE; ++j) {
-    const int i = warp + kWarps * j;
-    if (i >= NG) break;
-    const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-    float v[8], sum = 0.f;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      // a row with a non-finite value: zeros (its scale is NaN)
-      v[2 * x] = bad ? 0.f : bf16_lo(w[x]) * down;
-      v[2 * x + 1] = bad ? 0.f : bf16_hi(w[x]) * down;
-      sum += v[2 * x] + v[2 * x + 1];
+    for (int j = 0; j < MINE; ++j) {
+      const int i = warp + kWarps * j;
+      raw[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (g < G && i < NG) raw[j] = *reinterpret_cast<const uint4*>(rows + (long)g * a.q_head + 32 * i + 8 * t);
     }
-    sum += __shfl_xor_sync(kFull, sum, 1);
-    sum += __shfl_xor_sync(kFull, sum, 2);
-    if (t == 0) s.part[i][g] = sum;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      s.q[i][h][lane] = make_uint2(pack_half(v[2 * h], v[2 * h + 4]),
-                                   pack_half(v[2 * h + 1] * 0.0625f, v[2 * h + 5] * 0.0625f));
   }
-  if (warp == 0 && t == 0) s.scale[g] = bad ? __int_as_float(0x7fffffff) : ldexpf(a.scale_log2, e);
-  __syncthreads();
-  if (warp == 0) {
+
+  // the fragments into s; returns this lane's group sums as halves (high, low). Two barriers.
+  __device__ __forceinline__ uint2 prepare(Query<HD>& s, float scale_log2, int warp, int lane) const {
+    const int g = lane >> 2, t = lane & 3;
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+      const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) top = __vmaxu2(top, w[x] & 0x7fff7fffu);
+    }
+    top = max(top & 0xffffu, top >> 16);
+    top = max(top, __shfl_xor_sync(kFull, top, 1));
+    top = max(top, __shfl_xor_sync(kFull, top, 2));
+    if (t == 0) s.top[warp][g] = top;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kWarps; ++j) top = max(top, s.top[j][g]);
+    const bool bad = top >= 0x7f80u;   // a row with a non-finite value: zeros, and its scale is NaN
+    const int e = min(max((int)(top >> 7) - 127, -100), 127) - 9;   // at 2^-100 and below fewer bits are kept
+    const float down = kv4_pow2(-e);
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+      const int i = warp + kWarps * j;
+      if (i >= NG) break;
+      const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+      float v[8], sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        v[2 * x] = bad ? 0.f : bf16_lo(w[x]) * down;
+        v[2 * x + 1] = bad ? 0.f : bf16_hi(w[x]) * down;
+        sum += v[2 * x] + v[2 * x + 1];
+      }
+      sum += __shfl_xor_sync(kFull, sum, 1);
+      sum += __shfl_xor_sync(kFull, sum, 2);
+      if (t == 0) s.part[i][g] = sum;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        s.q[i][h][lane] = make_uint2(pack_half(v[2 * h], v[2 * h + 4]),
+                                     pack_half(v[2 * h + 1] * 0.0625f, v[2 * h + 5] * 0.0625f));
+    }
+    if (warp == 0 && t == 0) s.scale[g] = bad ? __int_as_float(0x7fffffff) : ldexpf(scale_log2, e);
+    __syncthreads();
     float a0 = 0.f, a1 = 0.f;
     if (2 * t < NG) a0 = s.part[2 * t][g], a1 = s.part[2 * t + 1][g];
     const uint32_t hi = pack_half(a0, a1);
     const float2 f = unpack_half(hi);
-    s.sums[lane] = make_uint2(hi, pack_half(a0 - f.x, a1 - f.y));
+    return make_uint2(hi, pack_half(a0 - f.x, a1 - f.y));
   }
-  __syncthreads();
-}
+};
 
 template <int HD>
 struct Warp {
@@ -207,7 +213,7 @@ struct Warp {
     return query->q[i][h][lane_];
   }
 
-  __device__ __forceinline__ void start(const Query<HD>& s, int lane) {
+  __device__ __forceinline__ void start(const Query<HD>& s, uint2 sums, int lane) {
     query = &s;
     lane_ = lane;
     if constexpr (kHold) {
@@ -216,7 +222,7 @@ struct Warp {
 #pragma unroll
         for (int h = 0; h < 2; ++h) held[i][h] = s.q[i][h][lane];
     }
-    qs = s.sums[lane];
+    qs = sums;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       cs[c] = s.scale[2 * (lane & 3) + c];
@@ -400,6 +406,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.hq / a.c.hkv;
   allow_next();
+  QueryLoad<HD> loading;                           // in flight while the position and the page ids are fetched
+  loading.load(a, a.q + (long)r * a.q_row + (long)g * G * a.q_head, G, warp, lane);
   const int p = a.pos[r];
   if (p < 0 || p >= a.c.rows[sq]) {
     if (p >= 0 && s == 0 && g == 0 && threadIdx.x == 0) record_error(a.err, kErrBadIndex);
@@ -450,9 +458,9 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
     issue();
   }
   __syncwarp();
-  load_query<HD>(query, a, a.q + (long)r * a.q_row + (long)g * G * a.q_head, G, warp, lane);
+  const uint2 sums = loading.prepare(query, a.scale_log2, warp, lane);
   Warp<HD> w;
-  w.start(query, lane);
+  w.start(query, sums, lane);
   int stage = 0, phase = 0;
   for (int k = NB * warp; k < blocks; k += NB * kWarps) {
     if (!__all_sync(kFull, mbar_wait(bar + stage, phase, a.err, kErrTimeoutProducer))) {
