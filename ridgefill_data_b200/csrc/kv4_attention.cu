@@ -43,7 +43,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -52,7 +52,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 // the same with a zero accumulator
 __device__ __forceinline__ void mma_f16_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                             uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
@@ -60,7 +60,7 @@ __device__ __forceinline__ void mma_f16_new(float (&c)[4], uint32_t a0, uint32_t
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -258,18 +258,28 @@ struct Warp {
         uint32_t w[2][KW];
 #pragma unroll
         for (int r = 0; r < 2; ++r) lds<KW>(k + L::k_word(g + 8 * r, t, i0), w[r]);
+        // the groups' first products, then their second ones: no product waits for the one just issued
+        float acc[KW][4];
 #pragma unroll
-        for (int i = i0; i < i0 + KW; ++i) {
-          float acc[4];
-          uint32_t x = w[0][i - i0], z = w[1][i - i0];
-          const uint2 q0 = q(i, 0), q1 = q(i, 1);
-          mma_f16_new(acc, x & 0x000f000fu, z & 0x000f000fu, x & 0x00f000f0u, z & 0x00f000f0u, q0.x, q0.y);
-          x >>= 8, z >>= 8;
-          mma_f16(acc, x & 0x000f000fu, z & 0x000f000fu, x & 0x00f000f0u, z & 0x00f000f0u, q1.x, q1.y);
+        for (int j = 0; j < KW; ++j) {
+          const uint2 f = q(i0 + j, 0);
+          mma_f16_new(acc[j], w[0][j] & 0x000f000fu, w[1][j] & 0x000f000fu, w[0][j] & 0x00f000f0u, w[1][j] & 0x00f000f0u,
+                      f.x, f.y);
+        }
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+          const uint2 f = q(i0 + j, 1);
+          const uint32_t x = w[0][j] >> 8, z = w[1][j] >> 8;
+          mma_f16(acc[j], x & 0x000f000fu, z & 0x000f000fu, x & 0x00f000f0u, z & 0x00f000f0u, f.x, f.y);
+        }
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+          const int i = i0 + j;
           const float2 p0 = unpack_half(ks[0][i / 2]), p1 = unpack_half(ks[1][i / 2]);
           const float s0 = i & 1 ? p0.y : p0.x, s1 = i & 1 ? p1.y : p1.x;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[j] = i == 0 ? (j < 2 ? s0 : s1) * acc[j] : fmaf(j < 2 ? s0 : s1, acc[j], s[j]);
+          for (int x = 0; x < 4; ++x)
+            s[x] = i == 0 ? (x < 2 ? s0 : s1) * acc[j][x] : fmaf(x < 2 ? s0 : s1, acc[j][x], s[x]);
         }
       }
       uint32_t m0 = 0, m1 = 0;
