@@ -149,7 +149,7 @@ void kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
     a.q_out_row = q_out->stride(0);
     a.q_out_head = q_out->stride(1);
   }
-  TORCH_CHECK(src.size(0) * (hq + 2 * c.hkv) < (1ll << 33), "kv4.append: too many rows");
+  TORCH_CHECK(src.size(0) * (hq + 2 * c.hkv) < (1ll << 31), "kv4.append: too many rows");
   if (T == 0) return;
   a.src = bf(src);
   a.src_row = src.stride(0);
@@ -185,7 +185,7 @@ void kv4_read(Tensor pool, std::vector<Tensor> pages, OptT row0, int64_t row0_ho
                 "kv4.read: k and v rows head_dim apart, 16-byte aligned, the same strides");
   }
   const int64_t n = k.size(2);
-  TORCH_CHECK(n < (1ll << 31) - 64 && R * n * c.hkv < (1ll << 33), "kv4.read: too many rows");
+  TORCH_CHECK(n < (1ll << 31) - 64 && (n / 16 + 2) * c.hkv < (1ll << 31) / rf::kKv4Seqs, "kv4.read: too many rows");
   rf::Kv4ReadArgs a{};
   if (R == 0) return;
   a.row0 = first_rows(row0, row0_host, c, n, "kv4.read");

@@ -1,12 +1,14 @@
 // Append to and read from the 4-bit K/V cache (layout: kv4.cuh).
 //
-// kv4_append_kernel  one warp per (row, q head | k head | v head), a lane holding hd / 32 consecutive values: head norm
-//                    and rotation (q, k), then q goes out in bf16 and k / v rows are quantised into their block.
-// kv4_read_kernel    one warp per (row, KV head): the values the codes stand for, rounded once to bf16.
+// kv4_append_kernel  a warp takes one row and a run of its heads (q | k | v), a lane holding hd / 32 consecutive values: head
+//                    norm and rotation (q, k), then q goes out in bf16 and k / v rows are quantised into their block.
+// kv4_read_kernel    one warp per block of 16 rows: the block to shared memory in 16-byte pieces, then row by row the values
+//                    the codes stand for, rounded once to bf16, a whole row per store instruction.
 //
 // Roundings are the bf16 model's (norm and each step of the rotation round to bf16), so a cached key is the 4-bit form
 // of the row the bf16 cache would hold. The norm's sum of squares and its root are taken in 64 bits: products of two
-// bf16 are exact there, so the row, and with it every code next to a border, does not depend on the order of the sum.
+// bf16 are exact there, so the row, and with it every code next to a border, does not depend on the order of the sum;
+// the products with the root are carried as two 32-bit numbers (46 bits).
 #include "kv4.cuh"
 
 #include "kernels.h"
@@ -19,68 +21,131 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 
-// Head norm (mode -1 none, 0 plain, 1 zero-centred) and rotate-half RoPE on [0, rot) at position p of one row.
+// 1 / sqrt(m) to about 50 bits: two Newton steps on the 22 bits of the single-precision root.
+__device__ __forceinline__ double inverse_root(double m) {
+  if (!(m > 1e-30 && m < 1e30)) return 1.0 / sqrt(m);
+  double y = (double)rsqrtf((float)m);
+  const double h = 0.5 * m;
+  y = y * fma(-h * y, y, 1.5);
+  return y * fma(-h * y, y, 1.5);
+}
+
+// A lane's hd / 32 consecutive values of a row as bf16 pairs.
 template <int PER>
-__device__ __forceinline__ void norm_rope(float (&v)[PER], const __nv_bfloat16* w, const Kv4AppendArgs& a, int p,
-                                          int lane) {
+struct Row {
+  uint32_t w[PER / 2];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    if constexpr (PER == 8) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    } else if constexpr (PER == 4) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = u.x, w[1] = u.y;
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    }
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* p) const {
+    if constexpr (PER == 8)
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (PER == 4)
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+  }
+  __device__ __forceinline__ float get(int j) const { return j & 1 ? bf16_hi(w[j / 2]) : bf16_lo(w[j / 2]); }
+};
+
+__device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2_rn(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t add_bf16(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hadd2_rn(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// A lane's part of the rotation at one position: its entries of the tables, and the lane of its partners.
+template <int PER>
+struct Turn {
+  Row<PER> c, s;          // s negative in the first half
+  int from;
+  bool in;
+
+  __device__ __forceinline__ void load(const Kv4AppendArgs& a, int p, int lane) {
+    const int h = a.rot / 2, i0 = lane * PER;   // h is a multiple of PER: a lane's values lie on one side of it
+    in = i0 < a.rot;
+    from = lane;
+    if (in) {
+      const bool low = i0 < h;
+      const int t0 = low ? i0 : i0 - h;
+      from = low ? lane + h / PER : lane - h / PER;
+      c.load(a.cos + (long)p * h + t0);
+      s.load(a.sin + (long)p * h + t0);
+#pragma unroll
+      for (int j = 0; j < PER / 2; ++j) s.w[j] ^= low ? 0x80008000u : 0u;
+    }
+  }
+  // rotate-half, each product and the sum rounded to bf16 (a sum of two bf16 rounds the same by way of fp32: it is
+  // exact there, or too far from its larger term to move it)
+  __device__ __forceinline__ void apply(Row<PER>& v) const {
+#pragma unroll
+    for (int j = 0; j < PER / 2; ++j) {
+      const uint32_t x = __shfl_sync(kFull, v.w[j], from);
+      const uint32_t y = add_bf16(mul_bf16(v.w[j], c.w[j]), mul_bf16(x, s.w[j]));
+      v.w[j] = in ? y : v.w[j];
+    }
+  }
+};
+
+// Head norm of one row of a warp: mode 0 plain, 1 zero-centred.
+template <int PER>
+__device__ __forceinline__ void norm(Row<PER>& row, const Row<PER>& w, int mode, double eps) {
   constexpr int HD = 32 * PER;
-  const int h = a.rot / 2, i0 = lane * PER;
-  float wv[PER], cv[PER], sv[PER];
+  double ss = 0.0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) wv[j] = cv[j] = sv[j] = 0.f;
-  if (a.norm_mode >= 0) kv4_load<PER>(w + i0, wv);
-  if (i0 < a.rot) {   // h is a multiple of PER: a lane's values lie on one side of it and inside rot
-    const int t0 = i0 < h ? i0 : i0 - h;
+  for (int j = 0; j < PER; ++j) ss = fma((double)row.get(j), (double)row.get(j), ss);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      cv[j] = __bfloat162float(a.cos[(long)p * h + t0 + j]);
-      sv[j] = __bfloat162float(a.sin[(long)p * h + t0 + j]);
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+  const double inv = inverse_root(ss * (1.0 / HD) + eps);
+  const float rh = (float)inv, rl = (float)(inv - (double)rh);
+  float y[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const float v = row.get(j);
+    float ph = rh, pl = rl;
+    if (mode == 1) {   // (1 + w) r as ph + pl
+      const float wh = 1.f + w.get(j), wl = w.get(j) - (wh - 1.f);
+      ph = rh * wh, pl = fmaf(rl, wh, fmaf(rh, wl, fmaf(rh, wh, -ph)));
     }
+    const float p = v * ph;
+    y[j] = p + fmaf(v, pl, fmaf(v, ph, -p));
   }
-  if (a.norm_mode >= 0) {
-    double ss = 0.0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) ss += (double)v[j] * (double)v[j];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-    const double inv = 1.0 / sqrt(ss / HD + a.eps);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const double f = (double)v[j] * inv;
-      v[j] = a.norm_mode == 0 ? kv4_bfr(kv4_bfr((float)f) * wv[j]) : kv4_bfr((float)(f * (1.0 + (double)wv[j])));
-    }
-  }
-  if (a.rot > 0) {
-    const int loff = h / PER;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const float up = __shfl_down_sync(kFull, v[j], loff);
-      const float dn = __shfl_up_sync(kFull, v[j], loff);
-      if (i0 + j < a.rot)
-        v[j] = i0 + j < h ? kv4_bfr(kv4_bfr(v[j] * cv[j]) + kv4_bfr(-up * sv[j]))
-                          : kv4_bfr(kv4_bfr(v[j] * cv[j]) + kv4_bfr(dn * sv[j]));
-    }
+  for (int j = 0; j < PER / 2; ++j) {
+    row.w[j] = pack_bf16x2(y[2 * j], y[2 * j + 1]);
+    if (mode == 0) row.w[j] = mul_bf16(row.w[j], w.w[j]);
   }
 }
 
 // One row of a warp quantised into row r of its block.
 template <int HD, bool IS_V>
-__device__ __forceinline__ void put_row(const float (&y)[HD / 32], uint8_t* block, int r, int lane) {
+__device__ __forceinline__ void put_row(const Row<HD / 32>& row, uint8_t* block, int r, int lane) {
   using L = Kv4L<HD>;
   constexpr int PER = L::PER;
   constexpr int LANES = 32 / PER;   // lanes of a group
   unsigned top = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
-  top = __reduce_max_sync(kFull, top);
-  const bool bad = top >= 0x5b800000u;   // 2^56 and above, infinities and NaN
-  int e = top == 0 ? 0 : (int)(top >> 23) - 127;
+  for (int j = 0; j < PER / 2; ++j) top = __vmaxu2(top, row.w[j] & 0x7fff7fffu);
+  top = __reduce_max_sync(kFull, max(top & 0xffffu, top >> 16));
+  const bool bad = top >= 0x5b80u;   // 2^56 and above, infinities and NaN
+  int e = top == 0 ? 0 : (int)(top >> 7) - 127;
   e = max(-kKv4Limit, min(kKv4Limit, e));
   const float size = kv4_pow2(-e);
   float z[PER], lo = INFINITY, hi = -INFINITY;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    z[j] = bad ? 0.f : y[j] * size;
+    z[j] = bad ? 0.f : row.get(j) * size;
     lo = fminf(lo, z[j]);
     hi = fmaxf(hi, z[j]);
   }
@@ -89,15 +154,29 @@ __device__ __forceinline__ void put_row(const float (&y)[HD / 32], uint8_t* bloc
     lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
   }
-  const __half s = __float2half_rn((hi - lo) / 15.f);
+  // (hi - lo) / 15 correctly rounded: the product with the rounded reciprocal and one correction by the exact
+  // remainder (P. Markstein, 1990)
+  const float d15 = hi - lo, q15 = d15 * (1.f / 15.f);
+  const __half s = __float2half_rn(fmaf(fmaf(-15.f, q15, d15), 1.f / 15.f, q15));
   const float mf = __half2float(__float2half_rn(lo)) + 0.f, sf = __half2float(s);   // + 0: a zero is kept as +0
   const __half m = __float2half_rn(mf);
-  uint32_t codes = 0;
+  // round((z - m) / s) by the reciprocal, which is within 2^-18 of the quotient (below 17); by the quotient itself where
+  // that could decide the rounding
+  const float inv = sf == 0.f ? 0.f : __fdividef(1.f, sf);
+  float c[PER], near = 0.f;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const float c = sf == 0.f ? 0.f : fminf(fmaxf(rintf((z[j] - mf) / sf), 0.f), 15.f);
-    codes |= (uint32_t)c << (4 * j);
+    c[j] = (z[j] - mf) * inv;
+    near = fmaxf(near, fabsf(c[j] - ((c[j] + 12582912.f) - 12582912.f)));   // distance to the nearest integer
   }
+  if (near > 0.4999f) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) c[j] = (z[j] - mf) / sf;
+  }
+  uint32_t codes = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    codes |= (__float_as_uint(fminf(fmaxf(c[j], 0.f), 15.f) + 12582912.f) & 15u) << (4 * j);
   const int i = lane / LANES, in = lane % LANES;   // group, lane in it
   if constexpr (!IS_V) {
     if constexpr (PER == 8)
@@ -124,123 +203,185 @@ __device__ __forceinline__ void put_row(const float (&y)[HD / 32], uint8_t* bloc
   if (lane == 0) block[(IS_V ? L::VE : L::KE) + r] = (uint8_t)(bad ? kKv4Mark : e + 127);
 }
 
-template <int HD>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendArgs a, int r0, long tasks) {
+// Warps of a block: 8 rows of one run of heads (down 0), or 8 runs of one row (few rows: down 1).
+template <int HD, int RUN>
+__global__ void __launch_bounds__(256, HD == 256 ? 3 : 4)
+    kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows, int down) {
   constexpr int PER = HD / 32;
-  const long task = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (task >= tasks) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = a.hq + 2 * a.c.hkv;
-  const long n = task / heads;             // row of this launch
-  const int head = (int)(task % heads);
-  const int sq = (int)(n / a.T), t = (int)(n % a.T);
+  const int n = down ? blockIdx.x : blockIdx.x * 8 + warp;   // row of this launch
+  const int head0 = (down ? blockIdx.y * 8 + warp : blockIdx.y) * RUN;
+  if (n >= rows || head0 >= heads) return;
+  const int sq = a.T == 1 ? n : n < a.T ? 0 : n / a.T, t = n - sq * a.T;
   const long src_row = (long)r0 * a.T + n;
-  const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
-  const long row = (long)first + t;
-  const int p = a.pos != nullptr ? __ldg(a.pos + src_row) : a.pos_offset >= 0 ? a.pos_offset + t : (int)row;
-  const bool skip = first < 0;
-  bool ok = !skip && row < a.c.rows[sq] && (a.rot == 0 || (p >= 0 && p < a.table_rows));
-  const __nv_bfloat16* src = a.src + src_row * a.src_row;
-  if (head < a.hq) {
-    float v[PER];
+  const __nv_bfloat16* src = a.src + src_row * a.src_row + lane * PER;
+  Row<PER> raw[RUN];                           // every head's values in flight at once
 #pragma unroll
-    for (int j = 0; j < PER; ++j) v[j] = 0.f;
-    if (ok) {
-      kv4_load<PER>(src + (long)head * a.q_stride + lane * PER, v);
-      norm_rope<PER>(v, a.q_norm, a, p, lane);
-    }
-    kv4_store<PER>(a.q_out + src_row * a.q_out_row + (long)head * a.q_out_head + lane * PER, v);
-  } else {
-    const int kh = head - a.hq;
-    const int g = kh < a.c.hkv ? kh : kh - a.c.hkv;
-    uint8_t* block = ok ? kv4_block<HD>(a.c, sq, g, (int)row) : nullptr;
-    if (block == nullptr) {
-      if (!skip && lane == 0) record_error(a.err, kErrBadIndex);
-      return;
-    }
-    float v[PER];
-    kv4_load<PER>(src + a.k_col + (long)kh * HD + lane * PER, v);
+  for (int x = 0; x < RUN; ++x) {
+    const int head = head0 + x;
+    if (head < heads) raw[x].load(src + (head < a.hq ? head * a.q_stride : a.k_col + (head - a.hq) * HD));
+  }
+  const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
+  const long at = (long)first + t;
+  const int row = (int)at;
+  const int p = a.pos != nullptr ? __ldg(a.pos + src_row) : a.pos_offset >= 0 ? a.pos_offset + t : row;
+  const bool skip = first < 0;
+  const bool ok = !skip && at < a.c.rows[sq] && (a.rot == 0 || (p >= 0 && p < a.table_rows));
+  uint8_t* block = nullptr;                    // the row's block of KV head 0
+  long pitch = 0;                              // between KV heads
+  if (ok && head0 + RUN > a.hq) {
+    const int page = a.page_shift >= 0 ? row >> a.page_shift : row / a.c.page_size;
+    const int id = __ldg(a.c.pages[sq] + page);
+    pitch = (long)(a.c.page_size / 16) * Kv4L<HD>::BYTES;
+    if (id >= 0 && id < a.c.num_pages)
+      block = a.c.pool + (long)id * a.c.hkv * pitch + ((row - page * a.c.page_size) >> 4) * Kv4L<HD>::BYTES;
+  }
+  Turn<PER> turn;
+  turn.in = false, turn.from = lane;
+  if (ok && a.rot > 0 && head0 < a.hq + a.c.hkv) turn.load(a, p, lane);
+  if (!skip && block == nullptr && head0 + RUN > a.hq && lane == 0) record_error(a.err, kErrBadIndex);
+#pragma unroll
+  for (int x = 0; x < RUN; ++x) {
+    const int head = head0 + x, kh = head - a.hq;
+    if (head >= heads) break;
+    Row<PER> v = raw[x];
     if (kh < a.c.hkv) {
-      norm_rope<PER>(v, a.k_norm, a, p, lane);
-      put_row<HD, false>(v, block, (int)row & 15, lane);
-    } else {
-      put_row<HD, true>(v, block, (int)row & 15, lane);
+      if (a.norm_mode >= 0) {
+        Row<PER> w;
+        w.load((kh < 0 ? a.q_norm : a.k_norm) + lane * PER);
+        norm<PER>(v, w, a.norm_mode, a.eps);
+      }
+      if (a.rot > 0) turn.apply(v);
+    }
+    if (kh < 0) {
+      if (!ok)
+#pragma unroll
+        for (int j = 0; j < PER / 2; ++j) v.w[j] = 0;
+      v.store(a.q_out + src_row * a.q_out_row + (long)head * a.q_out_head + lane * PER);
+    } else if (block != nullptr) {
+      if (kh < a.c.hkv)
+        put_row<HD, false>(v, block + kh * pitch, row & 15, lane);
+      else
+        put_row<HD, true>(v, block + (kh - a.c.hkv) * pitch, row & 15, lane);
     }
   }
 }
 
+constexpr int kReadWarps = 4;
+
 template <int HD>
-__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4ReadArgs a, int r0, long tasks) {
+__global__ void __launch_bounds__(kReadWarps * 32) kv4_read_kernel(const __grid_constant__ Kv4ReadArgs a, int r0,
+                                                                   int spans, long tasks) {
   using L = Kv4L<HD>;
-  constexpr int PER = L::PER;
-  constexpr int LANES = 32 / PER;
-  const long task = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  constexpr int PER = L::PER, LANES = 32 / PER, PIECES = L::BYTES / 16;
+  __shared__ uint4 held[kReadWarps][PIECES];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long task = (long)blockIdx.x * kReadWarps + warp;
   if (task >= tasks) return;
-  const int t = (int)(task % a.n);
-  const int g = (int)(task / a.n % a.c.hkv), sq = (int)(task / a.n / a.c.hkv);
+  const int x = (int)(task % spans);
+  const int gs = (int)(task / spans), g = gs % a.c.hkv, sq = gs / a.c.hkv;
   const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
-  const long row = (long)first + t;
-  float kv[PER], vv[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) kv[j] = vv[j] = 0.f;
+  // rows [lo, hi) of the block, in rows of the output behind t0
+  const int block0 = first < 0 ? 0 : first / 16;
+  const int t0 = (block0 + x) * 16 - (first < 0 ? 0 : first);   // output row of the block's row 0
+  const int lo = max(0, -t0), hi = min(16, a.n - t0);
+  if (lo >= hi) return;
+  const long row = (long)(block0 + x) * 16;
   const uint8_t* block = first >= 0 && row < a.c.rows[sq] ? kv4_block<HD>(a.c, sq, g, (int)row) : nullptr;
-  if (block != nullptr) {
-    const int r = (int)row & 15, i = lane / LANES, in = lane % LANES;
-    uint32_t kc, vc;
-    if constexpr (PER == 8) {
-      kc = *reinterpret_cast<const uint32_t*>(block + L::k_word(r, in, i));
-      vc = *reinterpret_cast<const uint16_t*>(block + L::v_chunk(r, 2 * in) + 2 * i) |
-           (uint32_t)*reinterpret_cast<const uint16_t*>(block + L::v_chunk(r, 2 * in + 1) + 2 * i) << 16;
-    } else if constexpr (PER == 4) {
-      kc = *reinterpret_cast<const uint16_t*>(block + L::k_word(r, in / 2, i) + 2 * (in & 1));
-      vc = *reinterpret_cast<const uint16_t*>(block + L::v_chunk(r, in) + 2 * i);
-    } else {
-      kc = block[L::k_word(r, in / 4, i) + (in & 3)];
-      vc = block[L::v_chunk(r, in / 2) + 2 * i + (in & 1)];
-    }
-    const int ka = r * L::NG + i, va = i * 16 + kv4_slot(r);
-    const float ks = __half2float(reinterpret_cast<const __half*>(block + L::KS)[ka]);
-    const float km = __half2float(reinterpret_cast<const __half*>(block + L::KM)[ka]);
-    const float vs = __half2float(reinterpret_cast<const __half*>(block + L::VS)[va]);
-    const float vm = __half2float(reinterpret_cast<const __half*>(block + L::VM)[va]);
-    const float ke = kv4_size(block[L::KE + r]), ve = kv4_size(block[L::VE + r]);
+  const long at = (long)(r0 + sq) * a.out_seq + (long)g * a.out_head + (long)t0 * HD + lane * PER;
+  if (block == nullptr) {
+    if (first >= 0 && lane == 0) record_error(a.err, kErrBadIndex);
+    float zero[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      kv[j] = ke * fmaf(ks, (float)(kc >> (4 * j) & 15), km);
-      vv[j] = ve * fmaf(vs, (float)(vc >> (4 * j) & 15), vm);
+    for (int j = 0; j < PER; ++j) zero[j] = 0.f;
+    for (int r = lo; r < hi; ++r) {
+      kv4_store<PER>(a.k + at + (long)r * HD, zero);
+      kv4_store<PER>(a.v + at + (long)r * HD, zero);
     }
-  } else if (first >= 0 && lane == 0) {
-    record_error(a.err, kErrBadIndex);
+    return;
   }
-  const long at = (long)(r0 + sq) * a.out_seq + (long)g * a.out_head + (long)t * HD + lane * PER;
-  kv4_store<PER>(a.k + at, kv);
-  kv4_store<PER>(a.v + at, vv);
+#pragma unroll
+  for (int j = 0; j < (PIECES + 31) / 32; ++j)
+    if (lane + 32 * j < PIECES) held[warp][lane + 32 * j] = __ldg(reinterpret_cast<const uint4*>(block) + lane + 32 * j);
+  __syncwarp();
+  const uint8_t* b = reinterpret_cast<const uint8_t*>(held[warp]);
+  const int i = lane / LANES, in = lane % LANES;
+#pragma unroll 4
+  for (int r = lo; r < hi; ++r) {
+    uint32_t c[2];
+    if constexpr (PER == 8) {
+      c[0] = *reinterpret_cast<const uint32_t*>(b + L::k_word(r, in, i));
+      c[1] = *reinterpret_cast<const uint16_t*>(b + L::v_chunk(r, 2 * in) + 2 * i) |
+             (uint32_t)*reinterpret_cast<const uint16_t*>(b + L::v_chunk(r, 2 * in + 1) + 2 * i) << 16;
+    } else if constexpr (PER == 4) {
+      c[0] = *reinterpret_cast<const uint16_t*>(b + L::k_word(r, in / 2, i) + 2 * (in & 1));
+      c[1] = *reinterpret_cast<const uint16_t*>(b + L::v_chunk(r, in) + 2 * i);
+    } else {
+      c[0] = b[L::k_word(r, in / 4, i) + (in & 3)];
+      c[1] = b[L::v_chunk(r, in / 2) + 2 * i + (in & 1)];
+    }
+    const int at_s[2] = {r * L::NG + i, i * 16 + kv4_slot(r)};
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float s = __half2float(reinterpret_cast<const __half*>(b + (x ? L::VS : L::KS))[at_s[x]]);
+      const float m = __half2float(reinterpret_cast<const __half*>(b + (x ? L::VM : L::KM))[at_s[x]]);
+      const float size = kv4_size(b[(x ? L::VE : L::KE) + r]);
+      float v[PER];
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        // the code as a number: 2^23 + c minus 2^23
+        const float f = __int_as_float(0x4b000000 | (c[x] >> (4 * j) & 15)) - 8388608.f;
+        v[j] = size * fmaf(s, f, m);
+      }
+      kv4_store<PER>((x ? a.v : a.k) + at + (long)r * HD, v);
+    }
+  }
 }
 
 }  // namespace
 
-void kv4_append(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) {
-  const long tasks = (long)seqs * a.T * (a.hq + 2 * a.c.hkv);
-  if (tasks <= 0) return;
-  const unsigned blocks = (unsigned)((tasks + 7) / 8);
-  switch (a.c.hd) {
-    case 64: kv4_append_kernel<64><<<blocks, 256, 0, stream>>>(a, r0, tasks); break;
-    case 128: kv4_append_kernel<128><<<blocks, 256, 0, stream>>>(a, r0, tasks); break;
-    case 256: kv4_append_kernel<256><<<blocks, 256, 0, stream>>>(a, r0, tasks); break;
-    default: throw std::runtime_error("kv4_append: head_dim 64 / 128 / 256");
-  }
+constexpr int kRun = 4;
+
+template <int HD>
+void launch_append(Kv4AppendArgs a, int r0, int rows, cudaStream_t stream) {
+  const int heads = a.hq + 2 * a.c.hkv;
+  // a warp takes one head while that leaves the GPU's 592 schedulers short of warps, else kRun: the row's table entries
+  // are fetched once for them and their loads are in flight together
+  const int run = (long)rows * heads >= 592l * 8 * kRun ? kRun : 1;
+  const int runs = (heads + run - 1) / run, down = rows < 8;
+  const dim3 grid(down ? rows : (rows + 7) / 8, down ? (runs + 7) / 8 : runs);
+  a.page_shift = -1;
+  for (int j = 4; j < 31; ++j)
+    if (a.c.page_size == 1 << j) a.page_shift = j;
+  if (run == 1)
+    kv4_append_kernel<HD, 1><<<grid, 256, 0, stream>>>(a, r0, rows, down);
+  else
+    kv4_append_kernel<HD, kRun><<<grid, 256, 0, stream>>>(a, r0, rows, down);
   count_launch();
 }
 
-void kv4_read(const Kv4ReadArgs& a, int r0, int seqs, cudaStream_t stream) {
-  const long tasks = (long)seqs * a.n * a.c.hkv;
-  if (tasks <= 0) return;
-  const unsigned blocks = (unsigned)((tasks + 7) / 8);
+void kv4_append(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) {
+  const long rows = (long)seqs * a.T;
+  if (rows <= 0) return;
   switch (a.c.hd) {
-    case 64: kv4_read_kernel<64><<<blocks, 256, 0, stream>>>(a, r0, tasks); break;
-    case 128: kv4_read_kernel<128><<<blocks, 256, 0, stream>>>(a, r0, tasks); break;
-    case 256: kv4_read_kernel<256><<<blocks, 256, 0, stream>>>(a, r0, tasks); break;
+    case 64: launch_append<64>(a, r0, (int)rows, stream); break;
+    case 128: launch_append<128>(a, r0, (int)rows, stream); break;
+    case 256: launch_append<256>(a, r0, (int)rows, stream); break;
+    default: throw std::runtime_error("kv4_append: head_dim 64 / 128 / 256");
+  }
+}
+
+void kv4_read(const Kv4ReadArgs& a, int r0, int seqs, cudaStream_t stream) {
+  // blocks that n rows can touch: known exactly for a host row, else one more
+  const int spans = a.row0 == nullptr ? (a.row0_host + a.n - 1) / 16 - a.row0_host / 16 + 1 : (a.n + 14) / 16 + 1;
+  const long tasks = (long)seqs * spans * a.c.hkv;
+  if (tasks <= 0 || a.n <= 0) return;
+  const unsigned blocks = (unsigned)((tasks + kReadWarps - 1) / kReadWarps);
+  switch (a.c.hd) {
+    case 64: kv4_read_kernel<64><<<blocks, kReadWarps * 32, 0, stream>>>(a, r0, spans, tasks); break;
+    case 128: kv4_read_kernel<128><<<blocks, kReadWarps * 32, 0, stream>>>(a, r0, spans, tasks); break;
+    case 256: kv4_read_kernel<256><<<blocks, kReadWarps * 32, 0, stream>>>(a, r0, spans, tasks); break;
     default: throw std::runtime_error("kv4_read: head_dim 64 / 128 / 256");
   }
   count_launch();

@@ -36,6 +36,7 @@ struct Kv4AppendArgs {
   int pos_offset;                 // or the cache row (pos_offset < 0)
   __nv_bfloat16* q_out;           // rotated q rows
   long q_out_row, q_out_head;
+  int page_shift;                 // log2 of the page size, -1 when it is no power of two (set by the launch)
   int* err;
 };
 void kv4_append(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream);
