@@ -1,7 +1,8 @@
 // Append to and read from the 4-bit K/V cache (layout: kv4.cuh).
 //
-// kv4_append_kernel  a warp takes one row and a run of its heads (q | k | v), a lane holding hd / 32 consecutive values: head
-//                    norm and rotation (q, k), then q goes out in bf16 and k / v rows are quantised into their block.
+// kv4_append_kernel  a warp per row and head (q | k | v), a lane holding hd / 32 consecutive values: head norm and rotation
+//                    (q, k), then q goes out in bf16 and k / v rows are quantised into their block.
+// kv4_append_rows_kernel  the same for many rows: 16 values a lane, 2 / 4 / 8 heads (hd 256 / 128 / 64) a warp.
 // kv4_read_kernel    one warp per block of 16 rows: the block to shared memory in 16-byte pieces, then row by row the values
 //                    the codes stand for, rounded once to bf16, a whole row per store instruction.
 //
@@ -19,6 +20,9 @@ namespace rf {
 
 namespace {
 
+#ifndef RF_ROWS
+#define RF_ROWS 64
+#endif
 constexpr unsigned kFull = 0xffffffffu;
 
 // 1 / sqrt(m) to about 50 bits: two Newton steps on the 22 bits of the single-precision root.
@@ -29,6 +33,74 @@ __device__ __forceinline__ double inverse_root(double m) {
   y = y * fma(-h * y, y, 1.5);
   return y * fma(-h * y, y, 1.5);
 }
+
+__device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2_rn(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t add_bf16(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hadd2_rn(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// 1 / sqrt(mean square + eps) as two floats, and a pair of values times it and the norm weight (mode 0 plain, 1
+// zero-centred), rounded to bf16 where the model rounds.
+struct Root {
+  float rh, rl;
+  __device__ __forceinline__ explicit Root(double m) {
+    const double inv = inverse_root(m);
+    rh = (float)inv, rl = (float)(inv - (double)rh);
+  }
+  __device__ __forceinline__ float times(float v, float w, int mode) const {
+    float ph = rh, pl = rl;
+    if (mode == 1) {   // (1 + w) r as ph + pl
+      const float wh = 1.f + w, wl = w - (wh - 1.f);
+      ph = rh * wh, pl = fmaf(rl, wh, fmaf(rh, wl, fmaf(rh, wh, -ph)));
+    }
+    const float p = v * ph;
+    return p + fmaf(v, pl, fmaf(v, ph, -p));
+  }
+  __device__ __forceinline__ uint32_t pair(uint32_t v, uint32_t w, int mode) const {
+    const uint32_t y = pack_bf16x2(times(bf16_lo(v), bf16_lo(w), mode), times(bf16_hi(v), bf16_hi(w), mode));
+    return mode == 0 ? mul_bf16(y, w) : y;
+  }
+};
+
+// The 16 steps of a group whose z lie in [lo, hi].
+struct Steps {
+  __half s, m;
+  float mf, sf;
+  __device__ __forceinline__ Steps(float lo, float hi) {
+    // (hi - lo) / 15 correctly rounded: the product with the rounded reciprocal and one correction by the exact
+    // remainder (P. Markstein, 1990)
+    const float d = hi - lo, q = d * (1.f / 15.f);
+    s = __float2half_rn(fmaf(fmaf(-15.f, q, d), 1.f / 15.f, q));
+    mf = __half2float(__float2half_rn(lo)) + 0.f;   // + 0: a zero is kept as +0
+    m = __float2half_rn(mf);
+    sf = __half2float(s);
+  }
+  // round((z - m) / s) by the reciprocal, which is within 2^-18 of the quotient (below 17); by the quotient itself where
+  // that could decide the rounding. N codes to words of 8.
+  template <int N>
+  __device__ __forceinline__ void codes(const float (&z)[N], uint32_t* words) const {
+    const float inv = sf == 0.f ? 0.f : __fdividef(1.f, sf);
+    float c[N], near = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      c[j] = (z[j] - mf) * inv;
+      near = fmaxf(near, fabsf(c[j] - ((c[j] + 12582912.f) - 12582912.f)));   // distance to the nearest integer
+    }
+    if (near > 0.4999f) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) c[j] = (z[j] - mf) / sf;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const uint32_t code = (__float_as_uint(fminf(fmaxf(c[j], 0.f), 15.f) + 12582912.f) & 15u) << (4 * (j & 7));
+      words[j / 8] = j & 7 ? words[j / 8] | code : code;
+    }
+  }
+};
 
 // A lane's hd / 32 consecutive values of a row as bf16 pairs.
 template <int PER>
@@ -55,15 +127,6 @@ struct Row {
   }
   __device__ __forceinline__ float get(int j) const { return j & 1 ? bf16_hi(w[j / 2]) : bf16_lo(w[j / 2]); }
 };
-
-__device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmul2_rn(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t add_bf16(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hadd2_rn(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 
 // A lane's part of the rotation at one position: its entries of the tables, and the lane of its partners.
 template <int PER>
@@ -107,25 +170,9 @@ __device__ __forceinline__ void norm(Row<PER>& row, const Row<PER>& w, int mode,
   for (int j = 0; j < PER; ++j) ss = fma((double)row.get(j), (double)row.get(j), ss);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-  const double inv = inverse_root(ss * (1.0 / HD) + eps);
-  const float rh = (float)inv, rl = (float)(inv - (double)rh);
-  float y[PER];
+  const Root r(ss * (1.0 / HD) + eps);
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const float v = row.get(j);
-    float ph = rh, pl = rl;
-    if (mode == 1) {   // (1 + w) r as ph + pl
-      const float wh = 1.f + w.get(j), wl = w.get(j) - (wh - 1.f);
-      ph = rh * wh, pl = fmaf(rl, wh, fmaf(rh, wl, fmaf(rh, wh, -ph)));
-    }
-    const float p = v * ph;
-    y[j] = p + fmaf(v, pl, fmaf(v, ph, -p));
-  }
-#pragma unroll
-  for (int j = 0; j < PER / 2; ++j) {
-    row.w[j] = pack_bf16x2(y[2 * j], y[2 * j + 1]);
-    if (mode == 0) row.w[j] = mul_bf16(row.w[j], w.w[j]);
-  }
+  for (int j = 0; j < PER / 2; ++j) row.w[j] = r.pair(row.w[j], w.w[j], mode);
 }
 
 // One row of a warp quantised into row r of its block.
@@ -154,29 +201,9 @@ __device__ __forceinline__ void put_row(const Row<HD / 32>& row, uint8_t* block,
     lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
   }
-  // (hi - lo) / 15 correctly rounded: the product with the rounded reciprocal and one correction by the exact
-  // remainder (P. Markstein, 1990)
-  const float d15 = hi - lo, q15 = d15 * (1.f / 15.f);
-  const __half s = __float2half_rn(fmaf(fmaf(-15.f, q15, d15), 1.f / 15.f, q15));
-  const float mf = __half2float(__float2half_rn(lo)) + 0.f, sf = __half2float(s);   // + 0: a zero is kept as +0
-  const __half m = __float2half_rn(mf);
-  // round((z - m) / s) by the reciprocal, which is within 2^-18 of the quotient (below 17); by the quotient itself where
-  // that could decide the rounding
-  const float inv = sf == 0.f ? 0.f : __fdividef(1.f, sf);
-  float c[PER], near = 0.f;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    c[j] = (z[j] - mf) * inv;
-    near = fmaxf(near, fabsf(c[j] - ((c[j] + 12582912.f) - 12582912.f)));   // distance to the nearest integer
-  }
-  if (near > 0.4999f) {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) c[j] = (z[j] - mf) / sf;
-  }
-  uint32_t codes = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j)
-    codes |= (__float_as_uint(fminf(fmaxf(c[j], 0.f), 15.f) + 12582912.f) & 15u) << (4 * j);
+  const Steps st(lo, hi);
+  uint32_t codes;
+  st.codes<PER>(z, &codes);
   const int i = lane / LANES, in = lane % LANES;   // group, lane in it
   if constexpr (!IS_V) {
     if constexpr (PER == 8)
@@ -197,30 +224,91 @@ __device__ __forceinline__ void put_row(const Row<HD / 32>& row, uint8_t* block,
   }
   if (in == 0) {
     const int at = IS_V ? i * 16 + kv4_slot(r) : r * L::NG + i;
-    reinterpret_cast<__half*>(block + (IS_V ? L::VS : L::KS))[at] = s;
-    reinterpret_cast<__half*>(block + (IS_V ? L::VM : L::KM))[at] = m;
+    reinterpret_cast<__half*>(block + (IS_V ? L::VS : L::KS))[at] = st.s;
+    reinterpret_cast<__half*>(block + (IS_V ? L::VM : L::KM))[at] = st.m;
   }
   if (lane == 0) block[(IS_V ? L::VE : L::KE) + r] = (uint8_t)(bad ? kKv4Mark : e + 127);
 }
 
-// Warps of a block: 8 rows of one run of heads (down 0), or 8 runs of one row (few rows: down 1).
-template <int HD, int RUN>
-__global__ void __launch_bounds__(256, HD == 256 ? 3 : 4)
+// A warp a row and head. Warps of a block: 8 rows of one head (down 0), or 8 heads of one row (few rows: down 1).
+template <int HD>
+__global__ void __launch_bounds__(256)
     kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows, int down) {
   constexpr int PER = HD / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = a.hq + 2 * a.c.hkv;
   const int n = down ? blockIdx.x : blockIdx.x * 8 + warp;   // row of this launch
-  const int head0 = (down ? blockIdx.y * 8 + warp : blockIdx.y) * RUN;
-  if (n >= rows || head0 >= heads) return;
+  const int head = down ? blockIdx.y * 8 + warp : blockIdx.y, kh = head - a.hq;
+  if (n >= rows || head >= heads) return;
   const int sq = a.T == 1 ? n : n < a.T ? 0 : n / a.T, t = n - sq * a.T;
   const long src_row = (long)r0 * a.T + n;
-  const __nv_bfloat16* src = a.src + src_row * a.src_row + lane * PER;
-  Row<PER> raw[RUN];                           // every head's values in flight at once
+  Row<PER> v, w;
+  v.load(a.src + src_row * a.src_row + lane * PER + (kh < 0 ? head * a.q_stride : a.k_col + kh * HD));
+  const bool normed = kh < a.c.hkv && a.norm_mode >= 0;
+  if (normed) w.load((kh < 0 ? a.q_norm : a.k_norm) + lane * PER);
+  const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
+  const long at = (long)first + t;
+  const int row = (int)at;
+  const int p = a.pos != nullptr ? __ldg(a.pos + src_row) : a.pos_offset >= 0 ? a.pos_offset + t : row;
+  const bool skip = first < 0;
+  const bool ok = !skip && at < a.c.rows[sq] && (a.rot == 0 || (p >= 0 && p < a.table_rows));
+  uint8_t* block = nullptr;
+  if (kh >= 0) {
+    if (ok) {
+      const int page = a.page_shift >= 0 ? row >> a.page_shift : row / a.c.page_size;
+      const int id = __ldg(a.c.pages[sq] + page);
+      const int g = kh < a.c.hkv ? kh : kh - a.c.hkv;
+      if (id >= 0 && id < a.c.num_pages)
+        block = a.c.pool +
+                (((long)id * a.c.hkv + g) * (a.c.page_size / 16) + ((row - page * a.c.page_size) >> 4)) * Kv4L<HD>::BYTES;
+    }
+    if (block == nullptr) {
+      if (!skip && lane == 0) record_error(a.err, kErrBadIndex);
+      return;
+    }
+  }
+  Turn<PER> turn;
+  turn.in = false, turn.from = lane;
+  if (ok && a.rot > 0 && kh < a.c.hkv) turn.load(a, p, lane);
+  if (normed) norm<PER>(v, w, a.norm_mode, a.eps);
+  if (a.rot > 0 && kh < a.c.hkv) turn.apply(v);
+  if (kh < 0) {
+    if (!ok)
 #pragma unroll
-  for (int x = 0; x < RUN; ++x) {
-    const int head = head0 + x;
-    if (head < heads) raw[x].load(src + (head < a.hq ? head * a.q_stride : a.k_col + (head - a.hq) * HD));
+      for (int j = 0; j < PER / 2; ++j) v.w[j] = 0;
+    v.store(a.q_out + src_row * a.q_out_row + (long)head * a.q_out_head + lane * PER);
+  } else if (kh < a.c.hkv) {
+    put_row<HD, false>(v, block, row & 15, lane);
+  } else {
+    put_row<HD, true>(v, block, row & 15, lane);
+  }
+}
+
+// The same for many rows: a lane holds 16 consecutive values (half a group), hd / 16 lanes a head, so a warp takes
+// 512 / hd heads of one row at once and what is done once a head or a group is done once for all of them. The rotation's
+// half must be whole lanes (rot / 2 a multiple of 16). blockIdx.y: the heads, q, then k, then v, in sets of a warp.
+template <int HD>
+__global__ void __launch_bounds__(256, 3) kv4_append_rows_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows) {
+  using L = Kv4L<HD>;
+  constexpr int LANES = HD / 16, HEADS = 32 / LANES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int j = lane % LANES;                  // lane of its head
+  const int n = blockIdx.x * 8 + warp;         // row of this launch
+  if (n >= rows) return;
+  const int q_sets = (a.hq + HEADS - 1) / HEADS, kv_sets = (a.c.hkv + HEADS - 1) / HEADS;
+  int set = blockIdx.y;
+  const int kind = set < q_sets ? 0 : set < q_sets + kv_sets ? 1 : 2;   // q, k, v
+  set -= kind == 0 ? 0 : kind == 1 ? q_sets : q_sets + kv_sets;
+  const int head = set * HEADS + lane / LANES;
+  const bool there = head < (kind == 0 ? a.hq : a.c.hkv);
+  const int sq = a.T == 1 ? n : n < a.T ? 0 : n / a.T, t = n - sq * a.T;
+  const long src_row = (long)r0 * a.T + n;
+  uint32_t v[8];
+  {
+    const int col = kind == 0 ? head * a.q_stride : a.k_col + (head + (kind == 2 ? a.c.hkv : 0)) * HD;
+    const uint4* src = reinterpret_cast<const uint4*>(a.src + src_row * a.src_row + (there ? col : 0) + 16 * j);
+    const uint4 x = __ldg(src), y = __ldg(src + 1);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
   }
   const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
   const long at = (long)first + t;
@@ -228,44 +316,103 @@ __global__ void __launch_bounds__(256, HD == 256 ? 3 : 4)
   const int p = a.pos != nullptr ? __ldg(a.pos + src_row) : a.pos_offset >= 0 ? a.pos_offset + t : row;
   const bool skip = first < 0;
   const bool ok = !skip && at < a.c.rows[sq] && (a.rot == 0 || (p >= 0 && p < a.table_rows));
-  uint8_t* block = nullptr;                    // the row's block of KV head 0
-  long pitch = 0;                              // between KV heads
-  if (ok && head0 + RUN > a.hq) {
-    const int page = a.page_shift >= 0 ? row >> a.page_shift : row / a.c.page_size;
-    const int id = __ldg(a.c.pages[sq] + page);
-    pitch = (long)(a.c.page_size / 16) * Kv4L<HD>::BYTES;
-    if (id >= 0 && id < a.c.num_pages)
-      block = a.c.pool + (long)id * a.c.hkv * pitch + ((row - page * a.c.page_size) >> 4) * Kv4L<HD>::BYTES;
-  }
-  Turn<PER> turn;
-  turn.in = false, turn.from = lane;
-  if (ok && a.rot > 0 && head0 < a.hq + a.c.hkv) turn.load(a, p, lane);
-  if (!skip && block == nullptr && head0 + RUN > a.hq && lane == 0) record_error(a.err, kErrBadIndex);
-#pragma unroll
-  for (int x = 0; x < RUN; ++x) {
-    const int head = head0 + x, kh = head - a.hq;
-    if (head >= heads) break;
-    Row<PER> v = raw[x];
-    if (kh < a.c.hkv) {
-      if (a.norm_mode >= 0) {
-        Row<PER> w;
-        w.load((kh < 0 ? a.q_norm : a.k_norm) + lane * PER);
-        norm<PER>(v, w, a.norm_mode, a.eps);
-      }
-      if (a.rot > 0) turn.apply(v);
+  uint8_t* block = nullptr;
+  if (kind > 0) {
+    if (ok) {
+      const int page = a.page_shift >= 0 ? row >> a.page_shift : row / a.c.page_size;
+      const int id = __ldg(a.c.pages[sq] + page);
+      if (id >= 0 && id < a.c.num_pages)
+        block = a.c.pool + (((long)id * a.c.hkv + head) * (a.c.page_size / 16) + ((row - page * a.c.page_size) >> 4)) * L::BYTES;
     }
-    if (kh < 0) {
-      if (!ok)
-#pragma unroll
-        for (int j = 0; j < PER / 2; ++j) v.w[j] = 0;
-      v.store(a.q_out + src_row * a.q_out_row + (long)head * a.q_out_head + lane * PER);
-    } else if (block != nullptr) {
-      if (kh < a.c.hkv)
-        put_row<HD, false>(v, block + kh * pitch, row & 15, lane);
-      else
-        put_row<HD, true>(v, block + (kh - a.c.hkv) * pitch, row & 15, lane);
+    if (block == nullptr) {                    // the same for the whole warp
+      if (!skip && lane == 0) record_error(a.err, kErrBadIndex);
+      return;
     }
   }
+  if (kind < 2 && a.norm_mode >= 0) {
+    double ss = 0.0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float l = bf16_lo(v[x]), h = bf16_hi(v[x]);
+      ss = fma((double)l, (double)l, ss);
+      ss = fma((double)h, (double)h, ss);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+    const Root r(ss * (1.0 / HD) + a.eps);
+    const uint4* wp = reinterpret_cast<const uint4*>((kind == 0 ? a.q_norm : a.k_norm) + 16 * j);
+    const uint4 x = __ldg(wp), y = __ldg(wp + 1);
+    const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = r.pair(v[x], w[x], a.norm_mode);
+  }
+  if (kind < 2 && a.rot > 0) {
+    const int h = a.rot / 32;                  // lanes of half the rotated values
+    const bool in = ok && j < 2 * h;
+    const int from = !in ? lane : j < h ? lane + h : lane - h;
+    uint32_t c[8], s[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) c[x] = s[x] = 0;
+    if (in) {
+      const long entry = (long)p * (a.rot / 2) + 16 * (j < h ? j : j - h);
+      const uint4* cp = reinterpret_cast<const uint4*>(a.cos + entry);
+      const uint4* sp = reinterpret_cast<const uint4*>(a.sin + entry);
+      const uint4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
+      c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+      s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+    }
+    const uint32_t sign = j < h ? 0x80008000u : 0u;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const uint32_t other = __shfl_sync(kFull, v[x], from);
+      const uint32_t turned = add_bf16(mul_bf16(v[x], c[x]), mul_bf16(other, s[x] ^ sign));
+      if (in) v[x] = turned;
+    }
+  }
+  if (kind == 0) {
+    if (!there) return;
+    uint4* dst = reinterpret_cast<uint4*>(a.q_out + src_row * a.q_out_row + (long)head * a.q_out_head + 16 * j);
+    dst[0] = ok ? make_uint4(v[0], v[1], v[2], v[3]) : make_uint4(0u, 0u, 0u, 0u);
+    dst[1] = ok ? make_uint4(v[4], v[5], v[6], v[7]) : make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
+  // quantise: the head's largest magnitude, then the group's ends over its two lanes
+  unsigned top = 0;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) top = __vmaxu2(top, v[x] & 0x7fff7fffu);
+  top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
+  const bool bad = top >= 0x5b80u;             // 2^56 and above, infinities and NaN
+  const int e = top == 0 ? 0 : max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
+  const float size = kv4_pow2(-e);
+  float z[16], lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    z[2 * x] = bad ? 0.f : bf16_lo(v[x]) * size;
+    z[2 * x + 1] = bad ? 0.f : bf16_hi(v[x]) * size;
+  }
+#pragma unroll
+  for (int x = 0; x < 16; ++x) lo = fminf(lo, z[x]), hi = fmaxf(hi, z[x]);
+  lo = fminf(lo, __shfl_xor_sync(kFull, lo, 1));
+  hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, 1));
+  const Steps st(lo, hi);
+  uint32_t codes[2];
+  st.codes<16>(z, codes);
+  if (!there) return;
+  const int r = row & 15, i = j / 2, half = j & 1;
+  if (kind == 1) {
+    *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * half, i)) = codes[0];
+    *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * half + 1, i)) = codes[1];
+  } else {
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<uint16_t*>(block + L::v_chunk(r, 4 * half + x) + 2 * i) = (uint16_t)(codes[x / 2] >> (16 * (x & 1)));
+  }
+  __half* params = reinterpret_cast<__half*>(block + (kind == 1 ? L::KS : L::VS));
+  // one lane of the group writes s, the other m (16 bytes of a row's, or hd / 2 halves, further)
+  params[(kind == 1 ? r * L::NG + i : i * 16 + kv4_slot(r)) + half * (HD / 2)] = half ? st.m : st.s;
+  if (j == 0) block[(kind == 1 ? L::KE : L::VE) + r] = (uint8_t)(bad ? kKv4Mark : e + 127);
 }
 
 constexpr int kReadWarps = 4;
@@ -341,23 +488,23 @@ __global__ void __launch_bounds__(kReadWarps * 32) kv4_read_kernel(const __grid_
 
 }  // namespace
 
-constexpr int kRun = 4;
-
 template <int HD>
 void launch_append(Kv4AppendArgs a, int r0, int rows, cudaStream_t stream) {
   const int heads = a.hq + 2 * a.c.hkv;
-  // a warp takes one head while that leaves the GPU's 592 schedulers short of warps, else kRun: the row's table entries
-  // are fetched once for them and their loads are in flight together
-  const int run = (long)rows * heads >= 592l * 8 * kRun ? kRun : 1;
-  const int runs = (heads + run - 1) / run, down = rows < 8;
-  const dim3 grid(down ? rows : (rows + 7) / 8, down ? (runs + 7) / 8 : runs);
   a.page_shift = -1;
   for (int j = 4; j < 31; ++j)
     if (a.c.page_size == 1 << j) a.page_shift = j;
-  if (run == 1)
-    kv4_append_kernel<HD, 1><<<grid, 256, 0, stream>>>(a, r0, rows, down);
-  else
-    kv4_append_kernel<HD, kRun><<<grid, 256, 0, stream>>>(a, r0, rows, down);
+  // many rows: a lane does four to sixteen times the values a warp-wide step's worth at once; few: a warp a head, which is
+  // the shorter way through one row
+  if (rows >= RF_ROWS && a.rot % 32 == 0) {
+    constexpr int HEADS = 512 / HD;
+    const int sets = (a.hq + HEADS - 1) / HEADS + 2 * ((a.c.hkv + HEADS - 1) / HEADS);
+    kv4_append_rows_kernel<HD><<<dim3((rows + 7) / 8, sets), 256, 0, stream>>>(a, r0, rows);
+  } else if (rows < 8) {
+    kv4_append_kernel<HD><<<dim3(rows, (heads + 7) / 8), 256, 0, stream>>>(a, r0, rows, 1);
+  } else {
+    kv4_append_kernel<HD><<<dim3((rows + 7) / 8, heads), 256, 0, stream>>>(a, r0, rows, 0);
+  }
   count_launch();
 }
 

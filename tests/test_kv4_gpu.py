@@ -58,6 +58,10 @@ APPEND = [
     (64, 3, 5, False, 0, 32, 48, [7, 40], 45),
     (64, 2, 4, True, 1, 64, 64, [0], 16),
     (128, 3, 0, False, 1, 64, 256, [100], 33),
+    (128, 3, 5, True, 1, 64, 48, [5, 90], 70),
+    (256, 3, 2, False, 0, 64, 128, [200], 80),
+    (64, 5, 1, False, 1, 16, 32, [3], 100),
+    (128, 2, 2, False, -1, 0, 128, [0], 64),
 ]
 
 
