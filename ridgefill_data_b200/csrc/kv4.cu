@@ -9,11 +9,12 @@
 // Roundings are the bf16 model's (norm and each step of the rotation round to bf16), so a cached key is the 4-bit form
 // of the row the bf16 cache would hold. The norm's sum of squares and its root are taken in 64 bits: products of two
 // bf16 are exact there, so the row, and with it every code next to a border, does not depend on the order of the sum;
-// the products with the root are carried as two 32-bit numbers (46 bits).
+// a key's products with the root are carried as two 32-bit numbers (46 bits).
 #include "kv4.cuh"
 
 #include "kernels.h"
 
+#include <algorithm>
 #include <stdexcept>
 
 namespace rf {
@@ -22,6 +23,7 @@ namespace {
 
 #ifndef RF_ROWS
 #define RF_ROWS 64
+#define RF_CT (148 * 6)
 #endif
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -43,15 +45,17 @@ __device__ __forceinline__ uint32_t add_bf16(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// 1 / sqrt(mean square + eps) as two floats, and a pair of values times it and the norm weight (mode 0 plain, 1
-// zero-centred), rounded to bf16 where the model rounds.
+// 1 / sqrt(mean square + eps), and a pair of values times it and the norm weight (mode 0 plain, 1 zero-centred), rounded
+// to bf16 where the model rounds. Products in two floats for a row that is quantised, in one for a query (within 2^-22).
 struct Root {
   float rh, rl;
   __device__ __forceinline__ explicit Root(double m) {
     const double inv = inverse_root(m);
     rh = (float)inv, rl = (float)(inv - (double)rh);
   }
+  template <bool FINE>
   __device__ __forceinline__ float times(float v, float w, int mode) const {
+    if constexpr (!FINE) return v * (mode == 1 ? rh * (1.f + w) : rh);
     float ph = rh, pl = rl;
     if (mode == 1) {   // (1 + w) r as ph + pl
       const float wh = 1.f + w, wl = w - (wh - 1.f);
@@ -60,45 +64,60 @@ struct Root {
     const float p = v * ph;
     return p + fmaf(v, pl, fmaf(v, ph, -p));
   }
+  template <bool FINE>
   __device__ __forceinline__ uint32_t pair(uint32_t v, uint32_t w, int mode) const {
-    const uint32_t y = pack_bf16x2(times(bf16_lo(v), bf16_lo(w), mode), times(bf16_hi(v), bf16_hi(w), mode));
+    const uint32_t y = pack_bf16x2(times<FINE>(bf16_lo(v), bf16_lo(w), mode), times<FINE>(bf16_hi(v), bf16_hi(w), mode));
     return mode == 0 ? mul_bf16(y, w) : y;
   }
 };
 
-// The 16 steps of a group whose z lie in [lo, hi].
+__device__ __forceinline__ uint32_t min_bf16(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max_bf16(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// The 16 steps of a group whose values lie in [lo, hi], in z = y * size.
 struct Steps {
   __half s, m;
-  float mf, sf;
-  __device__ __forceinline__ Steps(float lo, float hi) {
+  float mf, sf, size;
+  __device__ __forceinline__ Steps(float lo, float hi, float size_) : size(size_) {
     // (hi - lo) / 15 correctly rounded: the product with the rounded reciprocal and one correction by the exact
     // remainder (P. Markstein, 1990)
-    const float d = hi - lo, q = d * (1.f / 15.f);
+    const float d = hi * size - lo * size, q = d * (1.f / 15.f);
     s = __float2half_rn(fmaf(fmaf(-15.f, q, d), 1.f / 15.f, q));
-    mf = __half2float(__float2half_rn(lo)) + 0.f;   // + 0: a zero is kept as +0
+    mf = __half2float(__float2half_rn(lo * size)) + 0.f;   // + 0: a zero is kept as +0
     m = __float2half_rn(mf);
     sf = __half2float(s);
   }
-  // round((z - m) / s) by the reciprocal, which is within 2^-18 of the quotient (below 17); by the quotient itself where
-  // that could decide the rounding. N codes to words of 8.
+  // round((z - m) / s) of N values in bf16 pairs, to words of 8: the quotient by an approximate reciprocal and one
+  // correction by its remainder (Markstein again), the integer that an fp32 sum with 1.5 2^23 leaves in its low bits.
+  // Where s is so small that its own rounding can lead past 0 .. 15, held to them.
   template <int N>
-  __device__ __forceinline__ void codes(const float (&z)[N], uint32_t* words) const {
+  __device__ __forceinline__ void codes(const uint32_t* pairs, uint32_t* words) const {
+    constexpr float kBase = 12582912.f;            // its bits: 0x4b400000
     const float inv = sf == 0.f ? 0.f : __fdividef(1.f, sf);
-    float c[N], near = 0.f;
+    float c[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      c[j] = (z[j] - mf) * inv;
-      near = fmaxf(near, fabsf(c[j] - ((c[j] + 12582912.f) - 12582912.f)));   // distance to the nearest integer
+      const float d = fmaf(j & 1 ? bf16_hi(pairs[j / 2]) : bf16_lo(pairs[j / 2]), size, -mf);
+      const float q = d * inv;
+      c[j] = fmaf(fmaf(-q, sf, d), inv, q);
     }
-    if (near > 0.4999f) {
+    if (sf < 0x1p-13f) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) c[j] = (z[j] - mf) / sf;
+      for (int j = 0; j < N; ++j) c[j] = fminf(fmaxf(c[j], 0.f), 15.f);
     }
+    uint32_t base = 0;                             // the sum of the bases by 16^j
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const uint32_t code = (__float_as_uint(fminf(fmaxf(c[j], 0.f), 15.f) + 12582912.f) & 15u) << (4 * (j & 7));
-      words[j / 8] = j & 7 ? words[j / 8] | code : code;
-    }
+    for (int j = 0; j < (N < 8 ? N : 8); ++j) base += 0x4b400000u << (4 * j);
+#pragma unroll
+    for (int x = 0; x < (N + 7) / 8; ++x) words[x] = 0u - base;
+#pragma unroll
+    for (int j = 0; j < N; ++j) words[j / 8] += __float_as_uint(c[j] + kBase) << (4 * (j & 7));
   }
 };
 
@@ -163,7 +182,7 @@ struct Turn {
 
 // Head norm of one row of a warp: mode 0 plain, 1 zero-centred.
 template <int PER>
-__device__ __forceinline__ void norm(Row<PER>& row, const Row<PER>& w, int mode, double eps) {
+__device__ __forceinline__ void norm(Row<PER>& row, const Row<PER>& w, int mode, double eps, bool fine) {
   constexpr int HD = 32 * PER;
   double ss = 0.0;
 #pragma unroll
@@ -172,7 +191,8 @@ __device__ __forceinline__ void norm(Row<PER>& row, const Row<PER>& w, int mode,
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
   const Root r(ss * (1.0 / HD) + eps);
 #pragma unroll
-  for (int j = 0; j < PER / 2; ++j) row.w[j] = r.pair(row.w[j], w.w[j], mode);
+  for (int j = 0; j < PER / 2; ++j)
+    row.w[j] = fine ? r.pair<true>(row.w[j], w.w[j], mode) : r.pair<false>(row.w[j], w.w[j], mode);
 }
 
 // One row of a warp quantised into row r of its block.
@@ -188,22 +208,21 @@ __device__ __forceinline__ void put_row(const Row<HD / 32>& row, uint8_t* block,
   const bool bad = top >= 0x5b80u;   // 2^56 and above, infinities and NaN
   int e = top == 0 ? 0 : (int)(top >> 7) - 127;
   e = max(-kKv4Limit, min(kKv4Limit, e));
-  const float size = kv4_pow2(-e);
-  float z[PER], lo = INFINITY, hi = -INFINITY;
+  Row<PER> v = row;
+  if (bad)
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    z[j] = bad ? 0.f : row.get(j) * size;
-    lo = fminf(lo, z[j]);
-    hi = fmaxf(hi, z[j]);
-  }
+    for (int j = 0; j < PER / 2; ++j) v.w[j] = 0;
+  float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) lo = fminf(lo, v.get(j)), hi = fmaxf(hi, v.get(j));
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) {
     lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
   }
-  const Steps st(lo, hi);
+  const Steps st(lo, hi, kv4_pow2(-e));
   uint32_t codes;
-  st.codes<PER>(z, &codes);
+  st.codes<PER>(v.w, &codes);
   const int i = lane / LANES, in = lane % LANES;   // group, lane in it
   if constexpr (!IS_V) {
     if constexpr (PER == 8)
@@ -270,7 +289,7 @@ __global__ void __launch_bounds__(256)
   Turn<PER> turn;
   turn.in = false, turn.from = lane;
   if (ok && a.rot > 0 && kh < a.c.hkv) turn.load(a, p, lane);
-  if (normed) norm<PER>(v, w, a.norm_mode, a.eps);
+  if (normed) norm<PER>(v, w, a.norm_mode, a.eps, kh >= 0);
   if (a.rot > 0 && kh < a.c.hkv) turn.apply(v);
   if (kh < 0) {
     if (!ok)
@@ -284,135 +303,162 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// One lane's share of a row: 16 values of a head, and where the row belongs.
+struct Piece {
+  uint4 x, y;
+  int row, p, id;       // cache row (negative: the sequence is skipped), rotary position, page (K / V; -1: none)
+  bool ok;
+};
+
 // The same for many rows: a lane holds 16 consecutive values (half a group), hd / 16 lanes a head, so a warp takes
-// 512 / hd heads of one row at once and what is done once a head or a group is done once for all of them. The rotation's
-// half must be whole lanes (rot / 2 a multiple of 16). blockIdx.y: the heads, q, then k, then v, in sets of a warp.
-template <int HD>
-__global__ void __launch_bounds__(256, 3) kv4_append_rows_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows) {
+// 512 / hd heads of one row at once and what is done once a head or a group is done once for all of them; it walks down
+// the rows with the next one's loads in flight. The rotation's half must be whole lanes (rot / 2 a multiple of 16), a
+// page's rows a power of two. blockIdx.y: the heads, q, then k, then v, in sets of a warp.
+// KIND 0 q, 1 k, 2 v; MODE the head norm (-1 none).
+template <int HD, int KIND, int MODE, bool TURN>
+__device__ __forceinline__ void walk_rows(const Kv4AppendArgs& a, int r0, int rows, int set) {
   using L = Kv4L<HD>;
   constexpr int LANES = HD / 16, HEADS = 32 / LANES;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
   const int j = lane % LANES;                  // lane of its head
-  const int n = blockIdx.x * 8 + warp;         // row of this launch
-  if (n >= rows) return;
-  const int q_sets = (a.hq + HEADS - 1) / HEADS, kv_sets = (a.c.hkv + HEADS - 1) / HEADS;
-  int set = blockIdx.y;
-  const int kind = set < q_sets ? 0 : set < q_sets + kv_sets ? 1 : 2;   // q, k, v
-  set -= kind == 0 ? 0 : kind == 1 ? q_sets : q_sets + kv_sets;
   const int head = set * HEADS + lane / LANES;
-  const bool there = head < (kind == 0 ? a.hq : a.c.hkv);
-  const int sq = a.T == 1 ? n : n < a.T ? 0 : n / a.T, t = n - sq * a.T;
-  const long src_row = (long)r0 * a.T + n;
-  uint32_t v[8];
-  {
-    const int col = kind == 0 ? head * a.q_stride : a.k_col + (head + (kind == 2 ? a.c.hkv : 0)) * HD;
-    const uint4* src = reinterpret_cast<const uint4*>(a.src + src_row * a.src_row + (there ? col : 0) + 16 * j);
-    const uint4 x = __ldg(src), y = __ldg(src + 1);
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-  }
-  const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
-  const long at = (long)first + t;
-  const int row = (int)at;
-  const int p = a.pos != nullptr ? __ldg(a.pos + src_row) : a.pos_offset >= 0 ? a.pos_offset + t : row;
-  const bool skip = first < 0;
-  const bool ok = !skip && at < a.c.rows[sq] && (a.rot == 0 || (p >= 0 && p < a.table_rows));
-  uint8_t* block = nullptr;
-  if (kind > 0) {
-    if (ok) {
-      const int page = a.page_shift >= 0 ? row >> a.page_shift : row / a.c.page_size;
-      const int id = __ldg(a.c.pages[sq] + page);
-      if (id >= 0 && id < a.c.num_pages)
-        block = a.c.pool + (((long)id * a.c.hkv + head) * (a.c.page_size / 16) + ((row - page * a.c.page_size) >> 4)) * L::BYTES;
-    }
-    if (block == nullptr) {                    // the same for the whole warp
-      if (!skip && lane == 0) record_error(a.err, kErrBadIndex);
-      return;
-    }
-  }
-  if (kind < 2 && a.norm_mode >= 0) {
-    double ss = 0.0;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const float l = bf16_lo(v[x]), h = bf16_hi(v[x]);
-      ss = fma((double)l, (double)l, ss);
-      ss = fma((double)h, (double)h, ss);
-    }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-    const Root r(ss * (1.0 / HD) + a.eps);
-    const uint4* wp = reinterpret_cast<const uint4*>((kind == 0 ? a.q_norm : a.k_norm) + 16 * j);
+  const bool there = head < (KIND == 0 ? a.hq : a.c.hkv);
+  const int col = KIND == 0 ? head * a.q_stride : a.k_col + (head + (KIND == 2 ? a.c.hkv : 0)) * HD;
+  // the next row to fetch: n of the launch, t of sequence sq
+  const int step = gridDim.x * 8;
+  int n = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (n >= rows) return;
+  int sq = n / a.T, t = n - sq * a.T;
+  const __nv_bfloat16* src = a.src + ((long)r0 * a.T + n) * a.src_row + (there ? col : 0) + 16 * j;
+  const long src_step = step * a.src_row;
+  uint32_t w[8];
+  if constexpr (MODE >= 0) {
+    const uint4* wp = reinterpret_cast<const uint4*>((KIND == 0 ? a.q_norm : a.k_norm) + 16 * j);
     const uint4 x = __ldg(wp), y = __ldg(wp + 1);
-    const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = r.pair(v[x], w[x], a.norm_mode);
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
   }
-  if (kind < 2 && a.rot > 0) {
-    const int h = a.rot / 32;                  // lanes of half the rotated values
-    const bool in = ok && j < 2 * h;
-    const int from = !in ? lane : j < h ? lane + h : lane - h;
-    uint32_t c[8], s[8];
-#pragma unroll
-    for (int x = 0; x < 8; ++x) c[x] = s[x] = 0;
-    if (in) {
-      const long entry = (long)p * (a.rot / 2) + 16 * (j < h ? j : j - h);
-      const uint4* cp = reinterpret_cast<const uint4*>(a.cos + entry);
-      const uint4* sp = reinterpret_cast<const uint4*>(a.sin + entry);
-      const uint4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
-      c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
-      s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+  const int half = a.rot / 32;                 // lanes of half the rotated values
+  const bool inside = j < 2 * half, low = j < half;
+  const int entry = 16 * (low ? j : j - half);
+  const uint32_t sign = low ? 0x80008000u : 0u;
+  const int from = !inside ? lane : low ? lane + half : lane - half;
+
+  auto fetch = [&](int m) {
+    Piece f;
+    const uint4* at = reinterpret_cast<const uint4*>(src);
+    f.x = __ldg(at), f.y = __ldg(at + 1);
+    const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
+    const unsigned row = (unsigned)first + t;  // below 2^32: first < 2^31, t < 2^30
+    f.p = a.pos != nullptr ? __ldg(a.pos + (long)r0 * a.T + m) : a.pos_offset >= 0 ? a.pos_offset + t : (int)row;
+    f.ok = first >= 0 && row < (unsigned)a.c.rows[sq] && (a.rot == 0 || (unsigned)f.p < (unsigned)a.table_rows);
+    f.row = first < 0 ? -1 : (int)(row & 0x7fffffffu);
+    f.id = -1;
+    if (KIND > 0 && f.ok) f.id = __ldg(a.c.pages[sq] + (row >> a.page_shift));
+    src += src_step;
+    t += step;
+    while (t >= a.T) t -= a.T, ++sq;           // past the last row: not used
+    return f;
+  };
+
+  Piece next = fetch(n);
+  for (; n < rows; n += step) {
+    const Piece f = next;
+    uint4 c0, c1, s0, s1;
+    if constexpr (TURN) {
+      const long e = f.ok && inside ? (long)f.p * (a.rot / 2) + entry : 0;
+      const uint4* cp = reinterpret_cast<const uint4*>(a.cos + e);
+      const uint4* sp = reinterpret_cast<const uint4*>(a.sin + e);
+      c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
     }
-    const uint32_t sign = j < h ? 0x80008000u : 0u;
+    if (n + step < rows) next = fetch(n + step);
+    uint32_t v[8] = {f.x.x, f.x.y, f.x.z, f.x.w, f.y.x, f.y.y, f.y.z, f.y.w};
+    if (KIND > 0 && (f.id < 0 || f.id >= a.c.num_pages)) {   // the same for the whole warp
+      if (f.row >= 0 && lane == 0) record_error(a.err, kErrBadIndex);
+      continue;
+    }
+    if constexpr (MODE >= 0) {
+      double ss = 0.0;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const uint32_t other = __shfl_sync(kFull, v[x], from);
-      const uint32_t turned = add_bf16(mul_bf16(v[x], c[x]), mul_bf16(other, s[x] ^ sign));
-      if (in) v[x] = turned;
+      for (int x = 0; x < 8; ++x) {
+        const float l = bf16_lo(v[x]), h = bf16_hi(v[x]);
+        ss = fma((double)l, (double)l, ss);
+        ss = fma((double)h, (double)h, ss);
+      }
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+      const Root r(ss * (1.0 / HD) + a.eps);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[x] = r.template pair<KIND == 1>(v[x], w[x], MODE);
+    }
+    if constexpr (TURN) {
+      const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      const uint32_t s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const uint32_t other = __shfl_sync(kFull, v[x], from) ^ sign;
+        const uint32_t y = add_bf16(mul_bf16(v[x], c[x]), mul_bf16(other, s[x]));
+        v[x] = inside ? y : v[x];
+      }
+    }
+    if constexpr (KIND == 0) {
+      if (there) {
+        uint4* out = reinterpret_cast<uint4*>(a.q_out + ((long)r0 * a.T + n) * a.q_out_row + (long)head * a.q_out_head + 16 * j);
+        out[0] = f.ok ? make_uint4(v[0], v[1], v[2], v[3]) : make_uint4(0u, 0u, 0u, 0u);
+        out[1] = f.ok ? make_uint4(v[4], v[5], v[6], v[7]) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    } else {
+      // quantise: the head's largest magnitude, then the group's ends over its two lanes
+      unsigned top = 0;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) top = __vmaxu2(top, v[x] & 0x7fff7fffu);
+      top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
+      const bool bad = top >= 0x5b80u;         // 2^56 and above, infinities and NaN
+      if (bad)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = 0;
+      const int e = top == 0 ? 0 : max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
+      uint32_t least = v[0], most = v[0];
+#pragma unroll
+      for (int x = 1; x < 8; ++x) least = min_bf16(least, v[x]), most = max_bf16(most, v[x]);
+      least = min_bf16(least, __shfl_xor_sync(kFull, least, 1));
+      most = max_bf16(most, __shfl_xor_sync(kFull, most, 1));
+      const Steps st(fminf(bf16_lo(least), bf16_hi(least)), fmaxf(bf16_lo(most), bf16_hi(most)), kv4_pow2(-e));
+      uint32_t codes[2];
+      st.codes<16>(v, codes);
+      if (!there) continue;
+      const int r = f.row & 15;
+      uint8_t* block = a.c.pool + (((long)f.id * a.c.hkv + head) * (a.c.page_size / 16) +
+                                   ((f.row & (a.c.page_size - 1)) >> 4)) * L::BYTES;
+      const int i = j / 2, side = j & 1;
+      if constexpr (KIND == 1) {
+        *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * side, i)) = codes[0];
+        *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * side + 1, i)) = codes[1];
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          *reinterpret_cast<uint16_t*>(block + L::v_chunk(r, 4 * side + x) + 2 * i) = (uint16_t)(codes[x / 2] >> (16 * (x & 1)));
+      }
+      // one lane of the group writes s, the other m (hd / 2 halves further)
+      __half* params = reinterpret_cast<__half*>(block + (KIND == 1 ? L::KS : L::VS));
+      params[(KIND == 1 ? r * L::NG + i : i * 16 + kv4_slot(r)) + side * (HD / 2)] = side ? st.m : st.s;
+      if (j == 0) block[(KIND == 1 ? L::KE : L::VE) + r] = (uint8_t)(bad ? kKv4Mark : e + 127);
     }
   }
-  if (kind == 0) {
-    if (!there) return;
-    uint4* dst = reinterpret_cast<uint4*>(a.q_out + src_row * a.q_out_row + (long)head * a.q_out_head + 16 * j);
-    dst[0] = ok ? make_uint4(v[0], v[1], v[2], v[3]) : make_uint4(0u, 0u, 0u, 0u);
-    dst[1] = ok ? make_uint4(v[4], v[5], v[6], v[7]) : make_uint4(0u, 0u, 0u, 0u);
-    return;
-  }
-  // quantise: the head's largest magnitude, then the group's ends over its two lanes
-  unsigned top = 0;
-#pragma unroll
-  for (int x = 0; x < 8; ++x) top = __vmaxu2(top, v[x] & 0x7fff7fffu);
-  top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
-  const bool bad = top >= 0x5b80u;             // 2^56 and above, infinities and NaN
-  const int e = top == 0 ? 0 : max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
-  const float size = kv4_pow2(-e);
-  float z[16], lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-  for (int x = 0; x < 8; ++x) {
-    z[2 * x] = bad ? 0.f : bf16_lo(v[x]) * size;
-    z[2 * x + 1] = bad ? 0.f : bf16_hi(v[x]) * size;
-  }
-#pragma unroll
-  for (int x = 0; x < 16; ++x) lo = fminf(lo, z[x]), hi = fmaxf(hi, z[x]);
-  lo = fminf(lo, __shfl_xor_sync(kFull, lo, 1));
-  hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, 1));
-  const Steps st(lo, hi);
-  uint32_t codes[2];
-  st.codes<16>(z, codes);
-  if (!there) return;
-  const int r = row & 15, i = j / 2, half = j & 1;
-  if (kind == 1) {
-    *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * half, i)) = codes[0];
-    *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * half + 1, i)) = codes[1];
-  } else {
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      *reinterpret_cast<uint16_t*>(block + L::v_chunk(r, 4 * half + x) + 2 * i) = (uint16_t)(codes[x / 2] >> (16 * (x & 1)));
-  }
-  __half* params = reinterpret_cast<__half*>(block + (kind == 1 ? L::KS : L::VS));
-  // one lane of the group writes s, the other m (16 bytes of a row's, or hd / 2 halves, further)
-  params[(kind == 1 ? r * L::NG + i : i * 16 + kv4_slot(r)) + half * (HD / 2)] = half ? st.m : st.s;
-  if (j == 0) block[(kind == 1 ? L::KE : L::VE) + r] = (uint8_t)(bad ? kKv4Mark : e + 127);
+}
+
+template <int HD, int MODE, bool TURN>
+__global__ void __launch_bounds__(256, MODE >= 0 ? 2 : 3) kv4_append_rows_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows) {
+  constexpr int HEADS = 512 / HD;
+  const int q_sets = (a.hq + HEADS - 1) / HEADS, kv_sets = (a.c.hkv + HEADS - 1) / HEADS;
+  const int set = blockIdx.y;
+  if (set < q_sets)
+    walk_rows<HD, 0, MODE, TURN>(a, r0, rows, set);
+  else if (set < q_sets + kv_sets)
+    walk_rows<HD, 1, MODE, TURN>(a, r0, rows, set - q_sets);
+  else
+    walk_rows<HD, 2, -1, false>(a, r0, rows, set - q_sets - kv_sets);
 }
 
 constexpr int kReadWarps = 4;
@@ -496,10 +542,19 @@ void launch_append(Kv4AppendArgs a, int r0, int rows, cudaStream_t stream) {
     if (a.c.page_size == 1 << j) a.page_shift = j;
   // many rows: a lane does four to sixteen times the values a warp-wide step's worth at once; few: a warp a head, which is
   // the shorter way through one row
-  if (rows >= RF_ROWS && a.rot % 32 == 0) {
+  if (rows >= RF_ROWS && a.rot % 32 == 0 && a.page_shift >= 0) {
     constexpr int HEADS = 512 / HD;
     const int sets = (a.hq + HEADS - 1) / HEADS + 2 * ((a.c.hkv + HEADS - 1) / HEADS);
-    kv4_append_rows_kernel<HD><<<dim3((rows + 7) / 8, sets), 256, 0, stream>>>(a, r0, rows);
+    const int walks = std::max(1, std::min((rows + 7) / 8, (RF_CT + sets - 1) / sets));
+    const dim3 grid(walks, sets);
+    switch ((a.norm_mode + 1) * 2 + (a.rot > 0)) {
+      case 0: kv4_append_rows_kernel<HD, -1, false><<<grid, 256, 0, stream>>>(a, r0, rows); break;
+      case 1: kv4_append_rows_kernel<HD, -1, true><<<grid, 256, 0, stream>>>(a, r0, rows); break;
+      case 2: kv4_append_rows_kernel<HD, 0, false><<<grid, 256, 0, stream>>>(a, r0, rows); break;
+      case 3: kv4_append_rows_kernel<HD, 0, true><<<grid, 256, 0, stream>>>(a, r0, rows); break;
+      case 4: kv4_append_rows_kernel<HD, 1, false><<<grid, 256, 0, stream>>>(a, r0, rows); break;
+      default: kv4_append_rows_kernel<HD, 1, true><<<grid, 256, 0, stream>>>(a, r0, rows); break;
+    }
   } else if (rows < 8) {
     kv4_append_kernel<HD><<<dim3(rows, (heads + 7) / 8), 256, 0, stream>>>(a, r0, rows, 1);
   } else {
