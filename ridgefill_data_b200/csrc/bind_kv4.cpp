@@ -106,6 +106,7 @@ void kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
   a.row0_host = (int)row0_host;
   TORCH_CHECK(norm_mode >= -1 && norm_mode <= 1, "kv4.append: norm_mode -1, 0 or 1");
   if (norm_mode >= 0) {
+    TORCH_CHECK(eps >= 1e-30 && eps <= 1e30, "kv4.append: a norm's eps lies between 1e-30 and 1e30");
     TORCH_CHECK(k_norm.has_value() && (hq == 0 || q_norm.has_value()), "kv4.append: norm weights");
     for (const OptT* w : {&q_norm, &k_norm})
       if (w->has_value()) {

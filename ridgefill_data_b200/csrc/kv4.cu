@@ -2,7 +2,7 @@
 //
 // kv4_append_kernel  a warp per row and head (q | k | v), a lane holding hd / 32 consecutive values: head norm and rotation
 //                    (q, k), then q goes out in bf16 and k / v rows are quantised into their block.
-// kv4_append_rows_kernel  the same for many rows: 16 values a lane, 2 / 4 / 8 heads (hd 256 / 128 / 64) a warp.
+// kv4_append_q_kernel, kv4_append_kv_kernel  the same for many rows (below).
 // kv4_read_kernel    one warp per block of 16 rows: the block to shared memory in 16-byte pieces, then row by row the values
 //                    the codes stand for, rounded once to bf16, a whole row per store instruction.
 //
@@ -14,17 +14,12 @@
 
 #include "kernels.h"
 
-#include <algorithm>
 #include <stdexcept>
 
 namespace rf {
 
 namespace {
 
-#ifndef RF_ROWS
-#define RF_ROWS 64
-#define RF_CT (148 * 6)
-#endif
 constexpr unsigned kFull = 0xffffffffu;
 
 // 1 / sqrt(m) to about 50 bits: two Newton steps on the 22 bits of the single-precision root.
@@ -43,6 +38,17 @@ __device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t add_bf16(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hadd2_rn(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// |x| of the lower and upper bf16 of a pair in 64 bits, by moving the exponent and the mantissa to their places (the
+// special-function unit's conversions would take most of a norm). Zero and subnormals come out as 2^-127 .. 2^-126:
+// their squares are nothing beside eps, which the caller holds to 1e-30 and more; infinities and NaN come out finite and
+// stay in the row itself.
+__device__ __forceinline__ double low_double(uint32_t w) {
+  return __hiloint2double((int)((w & 0x7fffu) * 8192u + 0x38000000u), 0);
+}
+__device__ __forceinline__ double high_double(uint32_t w) {
+  return __hiloint2double((int)(__umulhi(w & 0x7fff0000u, 0x20000000u) + 0x38000000u), 0);
 }
 
 // 1 / sqrt(mean square + eps), and a pair of values times it and the norm weight (mode 0 plain, 1 zero-centred), rounded
@@ -186,7 +192,10 @@ __device__ __forceinline__ void norm(Row<PER>& row, const Row<PER>& w, int mode,
   constexpr int HD = 32 * PER;
   double ss = 0.0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) ss = fma((double)row.get(j), (double)row.get(j), ss);
+  for (int j = 0; j < PER / 2; ++j) {
+    const double l = low_double(row.w[j]), h = high_double(row.w[j]);
+    ss = fma(h, h, fma(l, l, ss));
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
   const Root r(ss * (1.0 / HD) + eps);
@@ -303,162 +312,230 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// One lane's share of a row: 16 values of a head, and where the row belongs.
-struct Piece {
-  uint4 x, y;
-  int row, p, id;       // cache row (negative: the sequence is skipped), rotary position, page (K / V; -1: none)
+// Many rows: the queries and the cached rows go their own ways.
+//
+// kv4_append_q_kernel   a lane holds 8 values (16 bytes), so a warp's loads and stores are whole sectors whatever the head
+//                       size: 256 / hd heads of a row at a time, two times. The rotation's half is whole lanes (rot / 2 a
+//                       multiple of 8).
+// kv4_append_kv_kernel  a CTA per block of 16 cache rows and 512 / hd heads of K or of V: a lane holds 16 values (half a
+//                       group), hd / 16 lanes a head, so what is done once a head or a group is done for all its heads at
+//                       once; the block's bytes are put together in shared memory and leave as 16-byte pieces (row by row
+//                       they would be 24 partial sectors a row and head). A block that is only partly appended is written
+//                       in place, row by row. The rotation's half is whole lanes (rot / 2 a multiple of 16).
+struct Place {
+  int row, p;   // cache row (negative: the sequence is skipped), rotary position
   bool ok;
 };
+__device__ __forceinline__ Place place(const Kv4AppendArgs& a, int first, int sq, int t, long src_row) {
+  Place f;
+  const unsigned row = (unsigned)first + t;   // below 2^32: first < 2^31, t < 2^30
+  f.p = a.pos != nullptr ? __ldg(a.pos + src_row) : a.pos_offset >= 0 ? a.pos_offset + t : (int)row;
+  f.ok = first >= 0 && row < (unsigned)a.c.rows[sq] && (a.rot == 0 || (unsigned)f.p < (unsigned)a.table_rows);
+  f.row = first < 0 ? -1 : (int)(row & 0x7fffffffu);
+  return f;
+}
 
-// The same for many rows: a lane holds 16 consecutive values (half a group), hd / 16 lanes a head, so a warp takes
-// 512 / hd heads of one row at once and what is done once a head or a group is done once for all of them; it walks down
-// the rows with the next one's loads in flight. The rotation's half must be whole lanes (rot / 2 a multiple of 16), a
-// page's rows a power of two. blockIdx.y: the heads, q, then k, then v, in sets of a warp.
-// KIND 0 q, 1 k, 2 v; MODE the head norm (-1 none).
-template <int HD, int KIND, int MODE, bool TURN>
-__device__ __forceinline__ void walk_rows(const Kv4AppendArgs& a, int r0, int rows, int set) {
-  using L = Kv4L<HD>;
-  constexpr int LANES = HD / 16, HEADS = 32 / LANES;
-  const int lane = threadIdx.x & 31;
-  const int j = lane % LANES;                  // lane of its head
-  const int head = set * HEADS + lane / LANES;
-  const bool there = head < (KIND == 0 ? a.hq : a.c.hkv);
-  const int col = KIND == 0 ? head * a.q_stride : a.k_col + (head + (KIND == 2 ? a.c.hkv : 0)) * HD;
-  // the next row to fetch: n of the launch, t of sequence sq
-  const int step = gridDim.x * 8;
-  int n = blockIdx.x * 8 + (threadIdx.x >> 5);
+template <int HD, int MODE, bool TURN>
+__global__ void __launch_bounds__(256) kv4_append_q_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows) {
+  constexpr int LANES = HD / 8, HEADS = 32 / LANES;
+  const int lane = threadIdx.x & 31, j = lane % LANES;
+  const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (n >= rows) return;
-  int sq = n / a.T, t = n - sq * a.T;
-  const __nv_bfloat16* src = a.src + ((long)r0 * a.T + n) * a.src_row + (there ? col : 0) + 16 * j;
-  const long src_step = step * a.src_row;
-  uint32_t w[8];
-  if constexpr (MODE >= 0) {
-    const uint4* wp = reinterpret_cast<const uint4*>((KIND == 0 ? a.q_norm : a.k_norm) + 16 * j);
-    const uint4 x = __ldg(wp), y = __ldg(wp + 1);
-    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
+  const int head = blockIdx.y * 2 * HEADS + lane / LANES;   // and HEADS further
+  const long src_row = (long)r0 * a.T + n;
+  const __nv_bfloat16* src = a.src + src_row * a.src_row + 8 * j;
+  Row<8> v[2], w;
+  const bool there[2] = {head < a.hq, head + HEADS < a.hq};
+#pragma unroll
+  for (int x = 0; x < 2; ++x) v[x].load(src + (there[x] ? (head + x * HEADS) * a.q_stride : 0));
+  if constexpr (MODE >= 0) w.load(a.q_norm + 8 * j);
+  int sq = 0, t = n;
+  if (t >= a.T) sq = n / a.T, t = n - sq * a.T;
+  const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
+  const Place f = place(a, first, sq, t, src_row);
+  Turn<8> turn;
+  if constexpr (TURN) {
+    const int h = a.rot / 2, i0 = 8 * j;
+    const bool low = i0 < h;
+    turn.in = i0 < a.rot;
+    turn.from = !turn.in ? lane : low ? lane + h / 8 : lane - h / 8;
+    const long entry = f.ok && turn.in ? (long)f.p * h + (low ? i0 : i0 - h) : 0;
+    turn.c.load(a.cos + entry);
+    turn.s.load(a.sin + entry);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) turn.s.w[x] ^= low ? 0x80008000u : 0u;
   }
-  const int half = a.rot / 32;                 // lanes of half the rotated values
-  const bool inside = j < 2 * half, low = j < half;
-  const int entry = 16 * (low ? j : j - half);
-  const uint32_t sign = low ? 0x80008000u : 0u;
-  const int from = !inside ? lane : low ? lane + half : lane - half;
-
-  auto fetch = [&](int m) {
-    Piece f;
-    const uint4* at = reinterpret_cast<const uint4*>(src);
-    f.x = __ldg(at), f.y = __ldg(at + 1);
-    const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
-    const unsigned row = (unsigned)first + t;  // below 2^32: first < 2^31, t < 2^30
-    f.p = a.pos != nullptr ? __ldg(a.pos + (long)r0 * a.T + m) : a.pos_offset >= 0 ? a.pos_offset + t : (int)row;
-    f.ok = first >= 0 && row < (unsigned)a.c.rows[sq] && (a.rot == 0 || (unsigned)f.p < (unsigned)a.table_rows);
-    f.row = first < 0 ? -1 : (int)(row & 0x7fffffffu);
-    f.id = -1;
-    if (KIND > 0 && f.ok) f.id = __ldg(a.c.pages[sq] + (row >> a.page_shift));
-    src += src_step;
-    t += step;
-    while (t >= a.T) t -= a.T, ++sq;           // past the last row: not used
-    return f;
-  };
-
-  Piece next = fetch(n);
-  for (; n < rows; n += step) {
-    const Piece f = next;
-    uint4 c0, c1, s0, s1;
-    if constexpr (TURN) {
-      const long e = f.ok && inside ? (long)f.p * (a.rot / 2) + entry : 0;
-      const uint4* cp = reinterpret_cast<const uint4*>(a.cos + e);
-      const uint4* sp = reinterpret_cast<const uint4*>(a.sin + e);
-      c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
-    }
-    if (n + step < rows) next = fetch(n + step);
-    uint32_t v[8] = {f.x.x, f.x.y, f.x.z, f.x.w, f.y.x, f.y.y, f.y.z, f.y.w};
-    if (KIND > 0 && (f.id < 0 || f.id >= a.c.num_pages)) {   // the same for the whole warp
-      if (f.row >= 0 && lane == 0) record_error(a.err, kErrBadIndex);
-      continue;
-    }
-    if constexpr (MODE >= 0) {
+  if constexpr (MODE >= 0) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
       double ss = 0.0;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const float l = bf16_lo(v[x]), h = bf16_hi(v[x]);
-        ss = fma((double)l, (double)l, ss);
-        ss = fma((double)h, (double)h, ss);
+      for (int y = 0; y < 4; ++y) {
+        const double l = low_double(v[x].w[y]), h = high_double(v[x].w[y]);
+        ss = fma(h, h, fma(l, l, ss));
       }
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
       const Root r(ss * (1.0 / HD) + a.eps);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) v[x] = r.template pair<KIND == 1>(v[x], w[x], MODE);
+      for (int y = 0; y < 4; ++y) v[x].w[y] = r.pair<false>(v[x].w[y], w.w[y], MODE);
     }
-    if constexpr (TURN) {
-      const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-      const uint32_t s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+  }
+  __nv_bfloat16* dst = a.q_out + src_row * a.q_out_row + 8 * j;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const uint32_t other = __shfl_sync(kFull, v[x], from) ^ sign;
-        const uint32_t y = add_bf16(mul_bf16(v[x], c[x]), mul_bf16(other, s[x]));
-        v[x] = inside ? y : v[x];
-      }
+  for (int x = 0; x < 2; ++x) {
+    if constexpr (TURN) turn.apply(v[x]);
+    if (!f.ok) v[x].w[0] = v[x].w[1] = v[x].w[2] = v[x].w[3] = 0;
+    if (there[x]) v[x].store(dst + (long)(head + x * HEADS) * a.q_out_head);
+  }
+}
+
+// One row of a warp's heads of K (or V), quantised to `block`, its head's block.
+template <int HD, bool IS_V, int MODE, bool TURN>
+__device__ __forceinline__ void cache_row(uint32_t (&v)[8], const Kv4AppendArgs& a, const uint32_t (&w)[8], const Place& f,
+                                          uint8_t* block, bool there, int r, int lane) {
+  using L = Kv4L<HD>;
+  constexpr int LANES = HD / 16;
+  const int j = lane % LANES;                  // lane of its head
+  if constexpr (MODE >= 0) {
+    double ss = 0.0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const double l = low_double(v[x]), h = high_double(v[x]);
+      ss = fma(h, h, fma(l, l, ss));
     }
-    if constexpr (KIND == 0) {
-      if (there) {
-        uint4* out = reinterpret_cast<uint4*>(a.q_out + ((long)r0 * a.T + n) * a.q_out_row + (long)head * a.q_out_head + 16 * j);
-        out[0] = f.ok ? make_uint4(v[0], v[1], v[2], v[3]) : make_uint4(0u, 0u, 0u, 0u);
-        out[1] = f.ok ? make_uint4(v[4], v[5], v[6], v[7]) : make_uint4(0u, 0u, 0u, 0u);
-      }
-    } else {
-      // quantise: the head's largest magnitude, then the group's ends over its two lanes
-      unsigned top = 0;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) top = __vmaxu2(top, v[x] & 0x7fff7fffu);
-      top = max(top & 0xffffu, top >> 16);
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+    const Root root(ss * (1.0 / HD) + a.eps);
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
-      const bool bad = top >= 0x5b80u;         // 2^56 and above, infinities and NaN
-      if (bad)
+    for (int x = 0; x < 8; ++x) v[x] = root.template pair<true>(v[x], w[x], MODE);
+  }
+  if constexpr (TURN) {
+    const int half = a.rot / 32;               // lanes of half the rotated values
+    const bool inside = j < 2 * half, low = j < half;
+    const int from = !inside ? lane : low ? lane + half : lane - half;
+    const uint32_t sign = low ? 0x80008000u : 0u;
+    const long e = inside ? (long)f.p * (a.rot / 2) + 16 * (low ? j : j - half) : 0;
+    const uint4* cp = reinterpret_cast<const uint4*>(a.cos + e);
+    const uint4* sp = reinterpret_cast<const uint4*>(a.sin + e);
+    const uint4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
+    const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+    const uint32_t s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] = 0;
-      const int e = top == 0 ? 0 : max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
-      uint32_t least = v[0], most = v[0];
-#pragma unroll
-      for (int x = 1; x < 8; ++x) least = min_bf16(least, v[x]), most = max_bf16(most, v[x]);
-      least = min_bf16(least, __shfl_xor_sync(kFull, least, 1));
-      most = max_bf16(most, __shfl_xor_sync(kFull, most, 1));
-      const Steps st(fminf(bf16_lo(least), bf16_hi(least)), fmaxf(bf16_lo(most), bf16_hi(most)), kv4_pow2(-e));
-      uint32_t codes[2];
-      st.codes<16>(v, codes);
-      if (!there) continue;
-      const int r = f.row & 15;
-      uint8_t* block = a.c.pool + (((long)f.id * a.c.hkv + head) * (a.c.page_size / 16) +
-                                   ((f.row & (a.c.page_size - 1)) >> 4)) * L::BYTES;
-      const int i = j / 2, side = j & 1;
-      if constexpr (KIND == 1) {
-        *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * side, i)) = codes[0];
-        *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * side + 1, i)) = codes[1];
-      } else {
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          *reinterpret_cast<uint16_t*>(block + L::v_chunk(r, 4 * side + x) + 2 * i) = (uint16_t)(codes[x / 2] >> (16 * (x & 1)));
-      }
-      // one lane of the group writes s, the other m (hd / 2 halves further)
-      __half* params = reinterpret_cast<__half*>(block + (KIND == 1 ? L::KS : L::VS));
-      params[(KIND == 1 ? r * L::NG + i : i * 16 + kv4_slot(r)) + side * (HD / 2)] = side ? st.m : st.s;
-      if (j == 0) block[(KIND == 1 ? L::KE : L::VE) + r] = (uint8_t)(bad ? kKv4Mark : e + 127);
+    for (int x = 0; x < 8; ++x) {
+      const uint32_t other = __shfl_sync(kFull, v[x], from) ^ sign;
+      const uint32_t y = add_bf16(mul_bf16(v[x], c[x]), mul_bf16(other, s[x]));
+      v[x] = inside ? y : v[x];
     }
+  }
+  // the head's largest magnitude, then the group's ends over its two lanes
+  unsigned top = 0;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) top = __vmaxu2(top, v[x] & 0x7fff7fffu);
+  top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
+  const bool bad = top >= 0x5b80u;             // 2^56 and above, infinities and NaN
+  if (bad)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = 0;
+  const int e = top == 0 ? 0 : max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
+  uint32_t least = v[0], most = v[0];
+#pragma unroll
+  for (int x = 1; x < 8; ++x) least = min_bf16(least, v[x]), most = max_bf16(most, v[x]);
+  least = min_bf16(least, __shfl_xor_sync(kFull, least, 1));
+  most = max_bf16(most, __shfl_xor_sync(kFull, most, 1));
+  const Steps st(fminf(bf16_lo(least), bf16_hi(least)), fmaxf(bf16_lo(most), bf16_hi(most)), kv4_pow2(-e));
+  uint32_t codes[2];
+  st.codes<16>(v, codes);
+  if (!there) return;
+  const int i = j / 2, side = j & 1;
+  if constexpr (!IS_V) {
+    *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * side, i)) = codes[0];
+    *reinterpret_cast<uint32_t*>(block + L::k_word(r, 2 * side + 1, i)) = codes[1];
+  } else {
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<uint16_t*>(block + L::v_chunk(r, 4 * side + x) + 2 * i) = (uint16_t)(codes[x / 2] >> (16 * (x & 1)));
+  }
+  // one lane of the group writes s, the other m (hd / 2 halves further)
+  __half* params = reinterpret_cast<__half*>(block + (IS_V ? L::VS : L::KS));
+  params[(IS_V ? i * 16 + kv4_slot(r) : r * L::NG + i) + side * (HD / 2)] = side ? st.m : st.s;
+  if (j == 0) block[(IS_V ? L::VE : L::KE) + r] = (uint8_t)(bad ? kKv4Mark : e + 127);
+}
+
+template <int HD, bool IS_V, int MODE, bool TURN>
+__device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs& a, int r0, int spans, int set) {
+  using L = Kv4L<HD>;
+  constexpr int LANES = HD / 16, HEADS = 32 / LANES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sq = blockIdx.x / spans, x = blockIdx.x - sq * spans;
+  const int head = set * HEADS + lane / LANES;
+  const bool there = head < a.c.hkv;
+  const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
+  if (first < 0) return;
+  const int block0 = first / 16 + x;           // the block of the sequence
+  // its rows: row r is row t0 + r of the call
+  const int t0 = block0 * 16 - first;          // above -16; past 2^31 only where no row is left
+  if (t0 >= a.T || (long)block0 * 16 >= (1l << 31)) return;
+  const __nv_bfloat16* src = a.src + a.k_col + ((there ? head : 0) + (IS_V ? a.c.hkv : 0)) * HD + 16 * (lane % LANES);
+  uint32_t v[2][8], w[8];
+  Place f[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = t0 + warp + 8 * u;
+    const bool mine = t >= 0 && t < a.T;
+    const long src_row = (long)(r0 + sq) * a.T + (mine ? t : 0);
+    const uint4* at = reinterpret_cast<const uint4*>(src + src_row * a.src_row);
+    const uint4 y = __ldg(at), z = __ldg(at + 1);
+    v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w, v[u][4] = z.x, v[u][5] = z.y, v[u][6] = z.z, v[u][7] = z.w;
+    f[u] = place(a, first, sq, t, src_row);
+    if (!mine) f[u].row = -1, f[u].ok = false;
+  }
+  if constexpr (MODE >= 0) {
+    const uint4* wp = reinterpret_cast<const uint4*>(a.k_norm + 16 * (lane % LANES));
+    const uint4 y = __ldg(wp), z = __ldg(wp + 1);
+    w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w, w[4] = z.x, w[5] = z.y, w[6] = z.z, w[7] = z.w;
+  }
+  const int per = a.c.page_size / 16;
+  int id = -1;
+  if (block0 * 16 < a.c.rows[sq]) id = __ldg(a.c.pages[sq] + block0 / per);
+  const bool page = id >= 0 && id < a.c.num_pages;
+  uint8_t* out = a.c.pool + (((long)(page ? id : 0) * a.c.hkv + set * HEADS) * per + block0 % per) * L::BYTES;   // head set * HEADS
+  const long pitch = (long)per * L::BYTES;
+  // every row here and in order: through shared memory
+  const bool whole = __syncthreads_and(f[0].ok && f[1].ok && page);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = warp + 8 * u;
+    if (!whole && !(f[u].ok && page)) {
+      if (f[u].row >= 0 && lane == 0) record_error(a.err, kErrBadIndex);
+      continue;
+    }
+    uint8_t* block = whole ? image + (lane / LANES) * L::BYTES : out + (lane / LANES) * pitch;
+    cache_row<HD, IS_V, MODE, TURN>(v[u], a, w, f[u], block, there, r, lane);
+  }
+  if (!whole) return;
+  __syncthreads();
+  // K: codes, s and m, exponents; V: the same, each behind K's
+  constexpr int CODES = HD / 2, PARAMS = HD / 8, PIECES = CODES + PARAMS + 1;
+  const int heads = min(HEADS, a.c.hkv - set * HEADS);
+  for (int y = threadIdx.x; y < heads * PIECES; y += 256) {
+    const int h = y / PIECES, piece = y - h * PIECES;
+    const int at = piece < CODES            ? (IS_V ? L::V : 0) + 16 * piece
+                   : piece < CODES + PARAMS ? (IS_V ? L::VS : L::KS) + 16 * (piece - CODES)
+                                            : (IS_V ? L::VE : L::KE);
+    *reinterpret_cast<uint4*>(out + h * pitch + at) = *reinterpret_cast<const uint4*>(image + h * L::BYTES + at);
   }
 }
 
 template <int HD, int MODE, bool TURN>
-__global__ void __launch_bounds__(256, MODE >= 0 ? 2 : 3) kv4_append_rows_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows) {
-  constexpr int HEADS = 512 / HD;
-  const int q_sets = (a.hq + HEADS - 1) / HEADS, kv_sets = (a.c.hkv + HEADS - 1) / HEADS;
-  const int set = blockIdx.y;
-  if (set < q_sets)
-    walk_rows<HD, 0, MODE, TURN>(a, r0, rows, set);
-  else if (set < q_sets + kv_sets)
-    walk_rows<HD, 1, MODE, TURN>(a, r0, rows, set - q_sets);
+__global__ void __launch_bounds__(256, 2) kv4_append_kv_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int spans) {
+  __shared__ __align__(16) uint8_t image[512 / HD * Kv4L<HD>::BYTES];
+  if (blockIdx.y & 1)
+    cache_block<HD, true, -1, false>(image, a, r0, spans, blockIdx.y / 2);
   else
-    walk_rows<HD, 2, -1, false>(a, r0, rows, set - q_sets - kv_sets);
+    cache_block<HD, false, MODE, TURN>(image, a, r0, spans, blockIdx.y / 2);
 }
 
 constexpr int kReadWarps = 4;
@@ -534,42 +611,53 @@ __global__ void __launch_bounds__(kReadWarps * 32) kv4_read_kernel(const __grid_
 
 }  // namespace
 
+template <int HD, int MODE, bool TURN>
+void launch_rows(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) {
+  const int rows = seqs * a.T;
+  if (a.hq > 0) {
+    kv4_append_q_kernel<HD, MODE, TURN>
+        <<<dim3((rows + 7) / 8, (a.hq + 512 / HD - 1) / (512 / HD)), 256, 0, stream>>>(a, r0, rows);
+    count_launch();
+  }
+  // blocks that T rows can touch: known exactly for a host row, else one more
+  const int spans = a.row0 == nullptr ? (int)(((long)a.row0_host + a.T - 1) / 16 - a.row0_host / 16 + 1) : (a.T + 14) / 16 + 1;
+  kv4_append_kv_kernel<HD, MODE, TURN>
+      <<<dim3(seqs * spans, 2 * ((a.c.hkv + 512 / HD - 1) / (512 / HD))), 256, 0, stream>>>(a, r0, spans);
+  count_launch();
+}
+
 template <int HD>
-void launch_append(Kv4AppendArgs a, int r0, int rows, cudaStream_t stream) {
-  const int heads = a.hq + 2 * a.c.hkv;
+void launch_append(Kv4AppendArgs a, int r0, int seqs, cudaStream_t stream) {
+  const int heads = a.hq + 2 * a.c.hkv, rows = seqs * a.T;
   a.page_shift = -1;
   for (int j = 4; j < 31; ++j)
     if (a.c.page_size == 1 << j) a.page_shift = j;
-  // many rows: a lane does four to sixteen times the values a warp-wide step's worth at once; few: a warp a head, which is
-  // the shorter way through one row
-  if (rows >= RF_ROWS && a.rot % 32 == 0 && a.page_shift >= 0) {
-    constexpr int HEADS = 512 / HD;
-    const int sets = (a.hq + HEADS - 1) / HEADS + 2 * ((a.c.hkv + HEADS - 1) / HEADS);
-    const int walks = std::max(1, std::min((rows + 7) / 8, (RF_CT + sets - 1) / sets));
-    const dim3 grid(walks, sets);
+  // From 64 rows of a sequence on (four blocks of the cache) the kernels for many rows; fewer: a warp a row and head, one
+  // launch and the shorter way through a row.
+  if (a.T >= 64 && a.rot % 32 == 0) {
     switch ((a.norm_mode + 1) * 2 + (a.rot > 0)) {
-      case 0: kv4_append_rows_kernel<HD, -1, false><<<grid, 256, 0, stream>>>(a, r0, rows); break;
-      case 1: kv4_append_rows_kernel<HD, -1, true><<<grid, 256, 0, stream>>>(a, r0, rows); break;
-      case 2: kv4_append_rows_kernel<HD, 0, false><<<grid, 256, 0, stream>>>(a, r0, rows); break;
-      case 3: kv4_append_rows_kernel<HD, 0, true><<<grid, 256, 0, stream>>>(a, r0, rows); break;
-      case 4: kv4_append_rows_kernel<HD, 1, false><<<grid, 256, 0, stream>>>(a, r0, rows); break;
-      default: kv4_append_rows_kernel<HD, 1, true><<<grid, 256, 0, stream>>>(a, r0, rows); break;
+      case 0: launch_rows<HD, -1, false>(a, r0, seqs, stream); break;
+      case 1: launch_rows<HD, -1, true>(a, r0, seqs, stream); break;
+      case 2: launch_rows<HD, 0, false>(a, r0, seqs, stream); break;
+      case 3: launch_rows<HD, 0, true>(a, r0, seqs, stream); break;
+      case 4: launch_rows<HD, 1, false>(a, r0, seqs, stream); break;
+      default: launch_rows<HD, 1, true>(a, r0, seqs, stream); break;
     }
-  } else if (rows < 8) {
-    kv4_append_kernel<HD><<<dim3(rows, (heads + 7) / 8), 256, 0, stream>>>(a, r0, rows, 1);
-  } else {
-    kv4_append_kernel<HD><<<dim3((rows + 7) / 8, heads), 256, 0, stream>>>(a, r0, rows, 0);
+    return;
   }
+  if (rows < 8)
+    kv4_append_kernel<HD><<<dim3(rows, (heads + 7) / 8), 256, 0, stream>>>(a, r0, rows, 1);
+  else
+    kv4_append_kernel<HD><<<dim3((rows + 7) / 8, heads), 256, 0, stream>>>(a, r0, rows, 0);
   count_launch();
 }
 
 void kv4_append(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) {
-  const long rows = (long)seqs * a.T;
-  if (rows <= 0) return;
+  if (seqs <= 0 || a.T <= 0) return;
   switch (a.c.hd) {
-    case 64: launch_append<64>(a, r0, (int)rows, stream); break;
-    case 128: launch_append<128>(a, r0, (int)rows, stream); break;
-    case 256: launch_append<256>(a, r0, (int)rows, stream); break;
+    case 64: launch_append<64>(a, r0, seqs, stream); break;
+    case 128: launch_append<128>(a, r0, seqs, stream); break;
+    case 256: launch_append<256>(a, r0, seqs, stream); break;
     default: throw std::runtime_error("kv4_append: head_dim 64 / 128 / 256");
   }
 }

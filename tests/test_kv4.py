@@ -101,6 +101,7 @@ APPEND_REFUSED = {
     "norm weight missing": (dict(norm_mode=0), "norm weights"),
     "norm weight size": (dict(norm_mode=0, k_norm=torch.zeros(64).bfloat16(), q_norm=torch.zeros(128).bfloat16()),
                          "norm weights"),
+    "norm eps": (dict(norm_mode=0, eps=0.0, k_norm=torch.zeros(128).bfloat16(), q_norm=torch.zeros(128).bfloat16()), "eps"),
     "rotary dims": (dict(rot=12), "rotary dims"),
     "rotary dims wide": (dict(rot=136), "rotary dims"),
     "no tables": (dict(rot=64), "RoPE tables"),
