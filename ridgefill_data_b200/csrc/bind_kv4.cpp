@@ -40,7 +40,7 @@ struct Cache {
     TORCH_CHECK((hd == 64 || hd == 128 || hd == 256) && pool.size(3) == 20 * hd + 32, op,
                 ": head_dim 64, 128 or 256 (blocks of 20 head_dim + 32 bytes)");
     TORCH_CHECK(pool.size(0) > 0 && pool.size(1) > 0 && pool.size(1) <= 65535 && pool.size(2) > 0 &&
-                    pool.size(0) < (1 << 30) && pool.size(2) < (1 << 26),
+                    pool.size(0) < (1 << 30) && pool.size(2) * pool.size(3) < (1ll << 31),
                 op, ": empty or oversized pool");
     num_pages = (int)pool.size(0);
     hkv = (int)pool.size(1);

@@ -9,7 +9,7 @@
 // Roundings are the bf16 model's (norm and each step of the rotation round to bf16), so a cached key is the 4-bit form
 // of the row the bf16 cache would hold. The norm's sum of squares and its root are taken in 64 bits: products of two
 // bf16 are exact there, so the row, and with it every code next to a border, does not depend on the order of the sum;
-// a key's products with the root are carried as two 32-bit numbers (46 bits).
+// its products with the root are carried as two 32-bit numbers (46 bits). A query is not quantised: 32 bits.
 #include "kv4.cuh"
 
 #include "kernels.h"
@@ -51,17 +51,15 @@ __device__ __forceinline__ double high_double(uint32_t w) {
   return __hiloint2double((int)(__umulhi(w & 0x7fff0000u, 0x20000000u) + 0x38000000u), 0);
 }
 
-// 1 / sqrt(mean square + eps), and a pair of values times it and the norm weight (mode 0 plain, 1 zero-centred), rounded
-// to bf16 where the model rounds. Products in two floats for a row that is quantised, in one for a query (within 2^-22).
+// 1 / sqrt(mean square + eps) of a key as two floats, and a pair of values times it and the norm weight (mode 0 plain, 1
+// zero-centred), rounded to bf16 where the model rounds.
 struct Root {
   float rh, rl;
   __device__ __forceinline__ explicit Root(double m) {
     const double inv = inverse_root(m);
     rh = (float)inv, rl = (float)(inv - (double)rh);
   }
-  template <bool FINE>
   __device__ __forceinline__ float times(float v, float w, int mode) const {
-    if constexpr (!FINE) return v * (mode == 1 ? rh * (1.f + w) : rh);
     float ph = rh, pl = rl;
     if (mode == 1) {   // (1 + w) r as ph + pl
       const float wh = 1.f + w, wl = w - (wh - 1.f);
@@ -70,16 +68,28 @@ struct Root {
     const float p = v * ph;
     return p + fmaf(v, pl, fmaf(v, ph, -p));
   }
-  template <bool FINE>
   __device__ __forceinline__ uint32_t pair(uint32_t v, uint32_t w, int mode) const {
-    const uint32_t y = pack_bf16x2(times<FINE>(bf16_lo(v), bf16_lo(w), mode), times<FINE>(bf16_hi(v), bf16_hi(w), mode));
+    const uint32_t y = pack_bf16x2(times(bf16_lo(v), bf16_lo(w), mode), times(bf16_hi(v), bf16_hi(w), mode));
     return mode == 0 ? mul_bf16(y, w) : y;
   }
 };
 
+// The same of a query, which is not quantised, in 32 bits: the arithmetic of head_norm_rope (norm.cu), bit for bit.
+__device__ __forceinline__ uint32_t query_pair(float inv, uint32_t v, uint32_t w, int mode) {
+  const float l = bf16_lo(v) * inv, h = bf16_hi(v) * inv;
+  return mode == 0 ? mul_bf16(pack_bf16x2(l, h), w)
+                   : pack_bf16x2(l * (1.f + bf16_lo(w)), h * (1.f + bf16_hi(w)));
+}
+
 __device__ __forceinline__ uint32_t min_bf16(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+// larger magnitude, NaN where either is
+__device__ __forceinline__ uint32_t top_bf16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
+  return r;
 }
 __device__ __forceinline__ uint32_t max_bf16(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
@@ -188,20 +198,30 @@ struct Turn {
 
 // Head norm of one row of a warp: mode 0 plain, 1 zero-centred.
 template <int PER>
-__device__ __forceinline__ void norm(Row<PER>& row, const Row<PER>& w, int mode, double eps, bool fine) {
+__device__ __forceinline__ void norm(Row<PER>& row, const Row<PER>& w, int mode, double eps, bool key) {
   constexpr int HD = 32 * PER;
-  double ss = 0.0;
+  if (key) {
+    double ss = 0.0;
 #pragma unroll
-  for (int j = 0; j < PER / 2; ++j) {
-    const double l = low_double(row.w[j]), h = high_double(row.w[j]);
-    ss = fma(h, h, fma(l, l, ss));
+    for (int j = 0; j < PER / 2; ++j) {
+      const double l = low_double(row.w[j]), h = high_double(row.w[j]);
+      ss = fma(h, h, fma(l, l, ss));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+    const Root r(ss * (1.0 / HD) + eps);
+#pragma unroll
+    for (int j = 0; j < PER / 2; ++j) row.w[j] = r.pair(row.w[j], w.w[j], mode);
+  } else {
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) ss = fmaf(row.get(j), row.get(j), ss);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+    const float inv = rsqrtf(ss / (float)HD + (float)eps);
+#pragma unroll
+    for (int j = 0; j < PER / 2; ++j) row.w[j] = query_pair(inv, row.w[j], w.w[j], mode);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-  const Root r(ss * (1.0 / HD) + eps);
-#pragma unroll
-  for (int j = 0; j < PER / 2; ++j)
-    row.w[j] = fine ? r.pair<true>(row.w[j], w.w[j], mode) : r.pair<false>(row.w[j], w.w[j], mode);
 }
 
 // One row of a warp quantised into row r of its block.
@@ -317,7 +337,7 @@ __global__ void __launch_bounds__(256)
 // kv4_append_q_kernel   a lane holds 8 values (16 bytes), so a warp's loads and stores are whole sectors whatever the head
 //                       size: 256 / hd heads of a row at a time, two times. The rotation's half is whole lanes (rot / 2 a
 //                       multiple of 8).
-// kv4_append_kv_kernel  a CTA per block of 16 cache rows and 512 / hd heads of K or of V: a lane holds 16 values (half a
+// kv4_append_kv_kernel  a CTA per block of 16 cache rows and 512 / hd heads of K or of V, a warp two rows: a lane holds 16 values (half a
 //                       group), hd / 16 lanes a head, so what is done once a head or a group is done for all its heads at
 //                       once; the block's bytes are put together in shared memory and leave as 16-byte pieces (row by row
 //                       they would be 24 partial sectors a row and head). A block that is only partly appended is written
@@ -368,17 +388,25 @@ __global__ void __launch_bounds__(256) kv4_append_q_kernel(const __grid_constant
   if constexpr (MODE >= 0) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      double ss = 0.0;
+      // the sums of the hd / 32 values that a lane holds when a warp takes one head, added across in that order too: the
+      // same bits as there
+      constexpr int PARTS = 256 / HD, PER = HD / 32;
+      float ss[PARTS];
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const double l = low_double(v[x].w[y]), h = high_double(v[x].w[y]);
-        ss = fma(h, h, fma(l, l, ss));
+      for (int y = 0; y < PARTS; ++y) {
+        ss[y] = 0.f;
+#pragma unroll
+        for (int z = 0; z < PER; ++z) ss[y] = fmaf(v[x].get(y * PER + z), v[x].get(y * PER + z), ss[y]);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) ss[y] += __shfl_xor_sync(kFull, ss[y], o);
       }
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-      const Root r(ss * (1.0 / HD) + a.eps);
+      for (int o = PARTS / 2; o > 0; o >>= 1)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) v[x].w[y] = r.pair<false>(v[x].w[y], w.w[y], MODE);
+        for (int y = 0; y < o; ++y) ss[y] += ss[y + o];
+      const float inv = rsqrtf(ss[0] / (float)HD + (float)a.eps);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) v[x].w[y] = query_pair(inv, v[x].w[y], w.w[y], MODE);
     }
   }
   __nv_bfloat16* dst = a.q_out + src_row * a.q_out_row + 8 * j;
@@ -408,7 +436,7 @@ __device__ __forceinline__ void cache_row(uint32_t (&v)[8], const Kv4AppendArgs&
     for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
     const Root root(ss * (1.0 / HD) + a.eps);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = root.template pair<true>(v[x], w[x], MODE);
+    for (int x = 0; x < 8; ++x) v[x] = root.pair(v[x], w[x], MODE);
   }
   if constexpr (TURN) {
     const int half = a.rot / 32;               // lanes of half the rotated values
@@ -429,9 +457,8 @@ __device__ __forceinline__ void cache_row(uint32_t (&v)[8], const Kv4AppendArgs&
     }
   }
   // the head's largest magnitude, then the group's ends over its two lanes
-  unsigned top = 0;
-#pragma unroll
-  for (int x = 0; x < 8; ++x) top = __vmaxu2(top, v[x] & 0x7fff7fffu);
+  unsigned top = top_bf16(top_bf16(top_bf16(v[0], v[1]), top_bf16(v[2], v[3])),
+                          top_bf16(top_bf16(v[4], v[5]), top_bf16(v[6], v[7])));
   top = max(top & 0xffffu, top >> 16);
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
@@ -464,12 +491,15 @@ __device__ __forceinline__ void cache_row(uint32_t (&v)[8], const Kv4AppendArgs&
   if (j == 0) block[(IS_V ? L::VE : L::KE) + r] = (uint8_t)(bad ? kKv4Mark : e + 127);
 }
 
+// kept out of line: the common page sizes are powers of two and branch past it
+__device__ __noinline__ int divide(int a, int b) { return a / b; }
+
 template <int HD, bool IS_V, int MODE, bool TURN>
-__device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs& a, int r0, int spans, int set) {
+__device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs& a, int r0, int set) {
   using L = Kv4L<HD>;
   constexpr int LANES = HD / 16, HEADS = 32 / LANES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sq = blockIdx.x / spans, x = blockIdx.x - sq * spans;
+  const int sq = blockIdx.z, x = blockIdx.x;
   const int head = set * HEADS + lane / LANES;
   const bool there = head < a.c.hkv;
   const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
@@ -479,7 +509,7 @@ __device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs&
   const int t0 = block0 * 16 - first;          // above -16; past 2^31 only where no row is left
   if (t0 >= a.T || (long)block0 * 16 >= (1l << 31)) return;
   const __nv_bfloat16* src = a.src + a.k_col + ((there ? head : 0) + (IS_V ? a.c.hkv : 0)) * HD + 16 * (lane % LANES);
-  uint32_t v[2][8], w[8];
+  uint32_t v[2][8], w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   Place f[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -498,22 +528,22 @@ __device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs&
     w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w, w[4] = z.x, w[5] = z.y, w[6] = z.z, w[7] = z.w;
   }
   const int per = a.c.page_size / 16;
+  const int nth = a.page_shift >= 0 ? block0 >> (a.page_shift - 4) : divide(block0, per);
   int id = -1;
-  if (block0 * 16 < a.c.rows[sq]) id = __ldg(a.c.pages[sq] + block0 / per);
+  if (block0 * 16 < a.c.rows[sq]) id = __ldg(a.c.pages[sq] + nth);
   const bool page = id >= 0 && id < a.c.num_pages;
-  uint8_t* out = a.c.pool + (((long)(page ? id : 0) * a.c.hkv + set * HEADS) * per + block0 % per) * L::BYTES;   // head set * HEADS
-  const long pitch = (long)per * L::BYTES;
+  const int pitch = per * L::BYTES;            // between KV heads (a page of a head is below 2^31 bytes)
+  uint8_t* out = a.c.pool + (long)((page ? id : 0) * (long)a.c.hkv + set * HEADS) * pitch + (block0 - nth * per) * L::BYTES;
   // every row here and in order: through shared memory
   const bool whole = __syncthreads_and(f[0].ok && f[1].ok && page);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int r = warp + 8 * u;
     if (!whole && !(f[u].ok && page)) {
       if (f[u].row >= 0 && lane == 0) record_error(a.err, kErrBadIndex);
       continue;
     }
-    uint8_t* block = whole ? image + (lane / LANES) * L::BYTES : out + (lane / LANES) * pitch;
-    cache_row<HD, IS_V, MODE, TURN>(v[u], a, w, f[u], block, there, r, lane);
+    uint8_t* block = whole ? image + (lane / LANES) * L::BYTES : out + (long)(lane / LANES) * pitch;
+    cache_row<HD, IS_V, MODE, TURN>(v[u], a, w, f[u], block, there, warp + 8 * u, lane);
   }
   if (!whole) return;
   __syncthreads();
@@ -525,17 +555,17 @@ __device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs&
     const int at = piece < CODES            ? (IS_V ? L::V : 0) + 16 * piece
                    : piece < CODES + PARAMS ? (IS_V ? L::VS : L::KS) + 16 * (piece - CODES)
                                             : (IS_V ? L::VE : L::KE);
-    *reinterpret_cast<uint4*>(out + h * pitch + at) = *reinterpret_cast<const uint4*>(image + h * L::BYTES + at);
+    *reinterpret_cast<uint4*>(out + (long)h * pitch + at) = *reinterpret_cast<const uint4*>(image + h * L::BYTES + at);
   }
 }
 
 template <int HD, int MODE, bool TURN>
-__global__ void __launch_bounds__(256, 2) kv4_append_kv_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int spans) {
+__global__ void __launch_bounds__(256, MODE == 1 ? 2 : 3) kv4_append_kv_kernel(const __grid_constant__ Kv4AppendArgs a, int r0) {
   __shared__ __align__(16) uint8_t image[512 / HD * Kv4L<HD>::BYTES];
   if (blockIdx.y & 1)
-    cache_block<HD, true, -1, false>(image, a, r0, spans, blockIdx.y / 2);
+    cache_block<HD, true, -1, false>(image, a, r0, blockIdx.y / 2);
   else
-    cache_block<HD, false, MODE, TURN>(image, a, r0, spans, blockIdx.y / 2);
+    cache_block<HD, false, MODE, TURN>(image, a, r0, blockIdx.y / 2);
 }
 
 constexpr int kReadWarps = 4;
@@ -622,7 +652,7 @@ void launch_rows(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) 
   // blocks that T rows can touch: known exactly for a host row, else one more
   const int spans = a.row0 == nullptr ? (int)(((long)a.row0_host + a.T - 1) / 16 - a.row0_host / 16 + 1) : (a.T + 14) / 16 + 1;
   kv4_append_kv_kernel<HD, MODE, TURN>
-      <<<dim3(seqs * spans, 2 * ((a.c.hkv + 512 / HD - 1) / (512 / HD))), 256, 0, stream>>>(a, r0, spans);
+      <<<dim3(spans, 2 * ((a.c.hkv + 512 / HD - 1) / (512 / HD)), seqs), 256, 0, stream>>>(a, r0);
   count_launch();
 }
 

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from ridgefill_data_b200.ops import kernels as K
 from ridgefill_data_b200.ops import kv4
 from ridgefill_data_b200.ops import oracle as ops
 from ridgefill_data_b200.ops._ext import check_errors, ext
@@ -94,20 +95,11 @@ def test_append_writes_the_oracles_bytes_and_no_others(case):
             ops.kv4_put(want[p, h, row % page // 16], row % 16, k[n, h].float(), v[n, h])
     assert torch.equal(pool.cpu(), want)
     if hq:
-        wq = src[:, :qw].reshape(R * T, hq, -1)[..., :hd]
-        want_q = ops.kv4_head_row(wq, norms[0], norm, 1e-6, cos, sin)
-        if norm < 0:
-            assert torch.equal(q.cpu().double(), want_q)
-        else:
-            # a query's normed values are 32-bit products within 2^-22 of the exact ones: one in about 2^-22 / 2^-9 rounds
-            # to the other neighbour, a step of 2^-7 of it; the rotation brings that step to itself and its partner, and
-            # every rounding after it (the weight's product, two products and the sum of the rotation) may move by one more
-            size = ops.kv4_head_row(wq, norms[0], norm, 1e-6).abs()
-            if rot:
-                h = rot // 2
-                size = torch.cat(((size[..., :h] + size[..., h:rot]).repeat(1, 1, 2), size[..., rot:]), -1)
-            off = (q.cpu().double() - want_q).abs()
-            assert (off <= 4 * 2.0 ** -7 * size).all() and (off > 0).double().mean() < 2e-3
+        want_q = torch.empty(R * T, hq, hd, dtype=torch.bfloat16, device=DEV)     # the bf16 path's query rows, bit for bit
+        K.head_norm_rope(src.to(DEV), hq, hd, 2 * hd if gated else hd, want_q, hd, hq * hd,
+                         norm_w=None if norm < 0 else norms[0].to(DEV), norm_mode=norm, eps=1e-6, tables=tables, rot=rot,
+                         pos=rows.to(DEV, torch.int32))
+        assert torch.equal(q, want_q)
     else:
         assert q is None
 
