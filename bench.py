@@ -203,6 +203,10 @@ def decode_bench(args):
     cfg = PRESETS[args.model]
     model = from_config(cfg, seed=0, device=device, backend="b200", std=0.02)
     rs = sorted({int(r) for r in args.decode.split(",") if r})
+    if args.kv_bits == 4:                  # every cache in one pool of 4-bit pages, as the server with --kv-bits 4
+        from ridgefill_data_b200.models.kvpool import KVPool
+        rows = args.decode_context + args.steps + 64
+        model.kv_pool = KVPool(model, max(rs) * -(-rows // 128), 128, bits=4)
     g = torch.Generator().manual_seed(0)
     caches, toks = [], []
     with torch.no_grad():
@@ -242,7 +246,7 @@ def decode_bench(args):
         print(json.dumps(dict(metric="greedy decode tokens/s (CUDA-graph step)", value=round(R * 1e3 / ms, 1),
                               unit="tokens/s", ms_per_step=round(ms, 3), sequences=R, steps=args.steps, warmup=3,
                               n_gpus=1, dtype="bf16", data="synthetic (seeded ids; random-init weights)",
-                              config=dict(model=args.model, context=args.decode_context),
+                              config=dict(model=args.model, context=args.decode_context, kv_bits=args.kv_bits),
                               weight_floor_ms=round(weight_bytes / (peaks.get("hbm_gbs", 6540.5) * 1e6), 2))),
               flush=True)
 
@@ -294,6 +298,8 @@ def main():
     ap.add_argument("--fit", action="store_true", help="time the ridge fit instead of the prefill (see fit_bench)")
     ap.add_argument("--decode", default="", help="time the decode step of these numbers of sequences instead of the "
                                                  "prefill, e.g. 1,3,8 (see decode_bench)")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=(4, 16),
+                    help="--decode: bits of a cached K/V value (4: a pool of 4-bit pages)")
     ap.add_argument("--decode-context", type=int, default=1024, help="prompt tokens of each decoding sequence")
     ap.add_argument("--fit-rows", type=int, default=839652)
     ap.add_argument("--fit-doc", type=int, default=8192, help="calibration document length (tokens)")

@@ -105,6 +105,30 @@ def _decode_attn(dev, a):
     return run, dict(flops=R * 4 * hq * hd * (n + 1), bytes=R * 2 * hkv * (n + 1) * hd * 2, shape=[R, n, hq, hkv, hd])
 
 
+def _decode_attn4(dev, a):
+    """The same decode row over 4-bit pages (append of the row, then attention): m sequences at position n."""
+    from .ops import kernels as K
+    from .ops import kv4
+    R, n = a.m or 8, a.n or 16384
+    hq, hkv, hd, rot = 24, 4, a.hd or 256, 64
+    held = n // 128 + 1
+    pool = kv4.pool(R * held, hkv, 128, hd, dev)
+    pages = list(torch.randperm(R * held, device=dev).int().split(held))
+    for p in pages:
+        kv4.append(torch.randn(n, 2 * hkv * hd, device=dev).bfloat16(), pool, p, 0)
+    qkv = torch.randn(R, hq * 2 * hd + 2 * hkv * hd, device=dev).bfloat16()
+    pos = torch.full((R,), n, dtype=torch.int32, device=dev)
+    qn, kn = ((torch.randn(hd, device=dev) * 0.1).bfloat16() for _ in range(2))
+    tables = K.rope_tables(1.0 / (1e7 ** (torch.arange(0, rot, 2, dtype=torch.float32) / rot)), n + 64, dev)
+    out = torch.empty(R, hq * hd, device=dev, dtype=torch.bfloat16)
+
+    def run():
+        q = kv4.append(qkv, pool, pages, pos, q_heads=hq, gated=True, q_norm=qn, k_norm=kn, norm_mode=1, tables=tables,
+                       rot=rot)
+        kv4.attention(q, pool, pages, pos, hd ** -0.5, out=out, gate=qkv[:, hd:], gate_head=2 * hd)
+    return run, dict(flops=R * 4 * hq * hd * (n + 1), bytes=R * hkv * (n + 1) * (1.25 * hd + 2), shape=[R, n, hq, hkv, hd])
+
+
 def _gdn_decode(dev, a):
     """One decode row of a 27B GDN layer (48 value heads of 128 x 128 fp32 state) for m sequences."""
     from .ops import kernels as K
@@ -124,14 +148,14 @@ def _gdn_decode(dev, a):
 
 
 WORKLOADS = {"gemm": _gemm, "attn": _attn, "gdn": _gdn, "moe": _moe, "gemv": _gemv, "decode_attn": _decode_attn,
-             "gdn_decode": _gdn_decode}
+             "decode_attn4": _decode_attn4, "gdn_decode": _gdn_decode}
 
 
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("workload", choices=sorted(WORKLOADS))
     ap.add_argument("--time", type=int, default=0, help="timed launches (0: two untimed launches only)")
-    ap.add_argument("--m", type=int, default=0, help="rows (gemm, gemv) or sequences (decode_attn, gdn_decode)")
+    ap.add_argument("--m", type=int, default=0, help="rows (gemm, gemv) or sequences (decode_attn, decode_attn4, gdn_decode)")
     ap.add_argument("--n", type=int, default=0, help="columns (gemm, gemv), tokens, or the decode position")
     ap.add_argument("--k", type=int, default=0)
     ap.add_argument("--hd", type=int, default=0)

@@ -19,6 +19,7 @@ import torch
 
 from ..ops import gemm as G
 from ..ops import kernels as K
+from ..ops import kv4
 from .base import KV_RESERVE
 from .hybrid import Hybrid
 from .llama import Llama
@@ -130,9 +131,13 @@ class _B200:
         c["k"], c["v"] = c["kbuf"][:, :n_new], c["vbuf"][:, :n_new]
 
     def _attend(self, i, q, c, nk, out, **kw):
-        """tcgen05 attention over cache entry c of layer i (contiguous buffers, or the pool's pages)."""
+        """tcgen05 attention over cache entry c of layer i (contiguous buffers, or the pool's pages; 4-bit pages are read
+        back in bf16 first)."""
         if self.kv_pool is not None:
             pool = self.kv_pool
+            if pool.bits == 4:
+                k, v = kv4.read(pool.kv[i], c["pages_dev"], nk)
+                return K.attention(q, k, v, nk, self.scale, out, **kw)
             return K.attention(q, pool.k[i], pool.v[i], nk, self.scale, out, pages=c["pages_dev"], **kw)
         return K.attention(q, c["kbuf"], c["vbuf"], nk, self.scale, out, **kw)
 
@@ -149,6 +154,10 @@ class _B200:
         p0, parr = self._span(pos)
         n0 = self._kv_reserve(c, m, i)
         tables = self.rope(p0 + m if parr is None else int(pos.max()) + 1)
+        if self.kv_pool is not None and self.kv_pool.bits == 4:
+            self._append4(i, kv_src, 0, c, n0, p0, parr, tables)
+            self._commit_kv(c, n0 + m)
+            return n0
         if self.kv_pool is not None:
             pool = self.kv_pool
             paged = dict(pages=c["pages_dev"], page_size=pool.page_size, page_stride=pool.page_stride, row0=n0)
@@ -166,6 +175,16 @@ class _B200:
         K.head_norm_rope(kv_src[:, hkv * hd:], hkv, hd, hd, vb[:, n0:], cap * hd, hd)
         self._commit_kv(c, n0 + m)
         return n0
+
+    def _append4(self, i, src, q_heads, c, n0, p0, parr, tables, q_out=None):
+        """Projected rows into the 4-bit pages of cache entry c from row n0 on (q heads first when q_heads: their rotated
+        rows go to q_out)."""
+        w = self.W[i]
+        rot = self.cfg.rot_dim
+        return kv4.append(src, self.kv_pool.kv[i], c["pages_dev"], n0, q_heads=q_heads, gated=self.cfg.gated_attn,
+                          q_norm=w.get("q_norm"), k_norm=w.get("k_norm"), norm_mode=self._qk_mode(), eps=self.eps,
+                          tables=tables if rot else None, rot=rot, pos=parr, pos_offset=p0 if parr is None else -1,
+                          q_out=q_out)
 
     def _attn_mix(self, i, h, pos, cache):
         """Attention block output added to h (new tensor) and the mixer output when asked."""
@@ -191,9 +210,15 @@ class _B200:
             self._attn_decode(i, qkv, torch.tensor([p0], dtype=torch.int32, device=self.device), [c], o)
             self._commit_kv(c, p0 + 1)
             return o
-        n0 = self._write_kv(i, qkv[:, qw:], pos, c)
         q = torch.empty(hq, n, hd, dtype=self.dtype, device=self.device)
         tables = self.rope(p0 + n if parr is None else int(pos.max()) + 1)
+        if self.kv_pool is not None and self.kv_pool.bits == 4:
+            n0 = self._kv_reserve(c, n, i)
+            self._append4(i, qkv, hq, c, n0, p0, parr, tables, q_out=q.transpose(0, 1))
+            self._commit_kv(c, n0 + n)
+            self._attend(i, q, c, n0 + n, o, q_start=n0, gate=qkv[:, hd:] if gated else None, gate_head=2 * hd)
+            return o
+        n0 = self._write_kv(i, qkv[:, qw:], pos, c)
         K.head_norm_rope(qkv, hq, hd, 2 * hd if gated else hd, q, n * hd, hd, norm_w=w.get("q_norm"),
                          norm_mode=self._qk_mode(), eps=self.eps, tables=tables, rot=self.cfg.rot_dim, pos=parr,
                          pos_offset=p0)
@@ -287,7 +312,11 @@ class _B200:
         return self.logits(h)
 
     def _attn_decode_ok(self):
-        """Whether the batched decode attention (csrc/attention_decode.cu) serves this model's attention layers."""
+        """Whether the batched decode attention (csrc/attention_decode.cu, or csrc/kv4_attention.cu over 4-bit pages) serves
+        this model's attention layers."""
+        pool = getattr(self, "kv_pool", None)
+        if pool is not None and pool.bits == 4:
+            return self.tp is None           # the pool checked the head shapes
         return self.tp is None and K.decode_attention_supported(self.head_dim, self.n_heads, self.n_kv,
                                                                 self.cfg.rot_dim)
 
@@ -298,6 +327,14 @@ class _B200:
         position. Writes out [R, hq * hd]."""
         w = self.W[i]
         hd, R = self.head_dim, len(entries)
+        if self.kv_pool is not None and self.kv_pool.bits == 4:
+            kv, pages, rot = self.kv_pool.kv[i], [c["pages_dev"] for c in entries], self.cfg.rot_dim
+            gated = self.cfg.gated_attn
+            q = kv4.append(qkv, kv, pages, pos_dev, q_heads=self.n_heads, gated=gated, q_norm=w.get("q_norm"),
+                           k_norm=w.get("k_norm"), norm_mode=self._qk_mode(), eps=self.eps,
+                           tables=self._rope_tables if rot else None, rot=rot)
+            return kv4.attention(q, kv, pages, pos_dev, self.scale, out=out, gate=qkv[:, hd:] if gated else None,
+                                 gate_head=2 * hd)
         if self.kv_pool is not None:
             pool = self.kv_pool
             k, v = [pool.k[i]] * R, [pool.v[i]] * R

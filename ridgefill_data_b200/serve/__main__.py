@@ -61,7 +61,7 @@ def build(args):
                            meta={"quality": qmode})}
     if getattr(args, "kv_pages", 0):
         from ..models.kvpool import KVPool
-        model.kv_pool = KVPool(model, args.kv_pages, getattr(args, "page_size", 128))
+        model.kv_pool = KVPool(model, args.kv_pages, getattr(args, "page_size", 128), bits=getattr(args, "kv_bits", 16))
     vocab = model.cfg.vocab
     props = dict(model=str(name), n_layers=model.n_layers, vocab=vocab, split=split, tail=args.tail,
                  backend=args.backend, interleave=args.interleave)
@@ -88,6 +88,8 @@ def main(argv=None):
                     help="serve every request from one paged K/V pool of this many pages per attention layer "
                          "(0: a contiguous cache per request)")
     ap.add_argument("--page-size", type=int, default=128, help="rows per K/V page (a multiple of 128)")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=(4, 16),
+                    help="bits of a cached value in the --kv-pages pool: 4 holds 3.2 times the tokens of 16")
     ap.add_argument("--interleave", type=int, default=4,
                     help="decode round every this many prefill layers (0: off; the period until --decode-gap-ms has "
                          "a measured prefill cost to work from)")
@@ -106,6 +108,8 @@ def main(argv=None):
     ap.add_argument("--host", default="127.0.0.1")
     ap.add_argument("--port", type=int, default=8080)
     a = ap.parse_args(argv)
+    if a.kv_bits != 16 and not a.kv_pages:
+        ap.error("--kv-bits 4 needs a page pool: give --kv-pages")
     if int(os.environ.get("WORLD_SIZE", "1")) > 1:
         return main_tp(a)
     from .app import Server, create_app

@@ -189,3 +189,34 @@ def test_attention_refuses():
                           gate_head=args["gate_head"])
     with pytest.raises(RuntimeError, match="CUDA device"):
         kv4.attention(q, pool, [table], pos, 0.1, gate=gate[:, 128:], gate_head=256)
+
+
+def test_4_bit_pool_on_the_cpu():
+    """Page bookkeeping and refusals of a pool of 4-bit pages."""
+    from types import SimpleNamespace
+
+    from ridgefill_data_b200.models.kvpool import KVPool, PoolExhausted
+    model = SimpleNamespace(head_dim=128, n_kv=2, n_heads=8, layer_types=["gdn", "attn", "attn"], cfg=SimpleNamespace(rot_dim=64),
+                            device=torch.device("cpu"), dtype=torch.bfloat16)
+    pool = KVPool(model, pages=6, page_size=128, bits=4)
+    assert pool.k is None and pool.v is None and pool.kv[1].shape == (6, 2, 8, kv4.block_bytes(128))
+    assert pool.bytes() == 2 * 6 * 2 * 8 * kv4.block_bytes(128)
+    entry = {}
+    pool.grow(2, entry, 129, "cpu")
+    assert len(entry["pages"]) == 2 and pool.free_pages(2) == 4
+    with pytest.raises(PoolExhausted):
+        pool.grow(2, {}, 700, "cpu")
+    pool.release([{}, {}, entry])
+    assert pool.free_pages(2) == 6
+    for over in (dict(head_dim=96), dict(n_heads=18), dict(n_heads=7), dict(cfg=SimpleNamespace(rot_dim=20))):
+        with pytest.raises(ValueError):
+            KVPool(SimpleNamespace(**{**vars(model), **over}), pages=2, bits=4)
+    for kw in (dict(bits=8), dict(bits=4, page_size=64), dict(bits=4, page_size=0)):
+        with pytest.raises(ValueError):
+            KVPool(model, pages=2, **kw)
+
+
+def test_server_flag_needs_a_pool():
+    from ridgefill_data_b200.serve.__main__ import main
+    with pytest.raises(SystemExit):
+        main(["--kv-bits", "4"])
