@@ -11,6 +11,8 @@
 
 #include "kv4.h"
 
+torch::Tensor& err_word(int dev);   // bindings.cpp: the per-device error word
+
 namespace {
 
 using at::Tensor;
@@ -58,6 +60,8 @@ struct Cache {
   // the last check before a launch, so that every other refusal holds on any device
   void on_gpu(const char* op) const { TORCH_CHECK(pool.is_cuda(), op, ": the cache must be on a CUDA device"); }
 
+  int* err() const { return err_word(pool.get_device()).data_ptr<int>(); }
+
   rf::Kv4Pages part(int64_t r0, int n) const {
     rf::Kv4Pages c{};
     c.pool = pool.data_ptr<uint8_t>();
@@ -87,13 +91,13 @@ const int* first_rows(const OptT& row0, int64_t host, const Cache& c, int64_t T,
   return nullptr;
 }
 
-void kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, int64_t row0_host, int64_t hq, bool gated,
-            OptT q_norm, OptT k_norm, int64_t norm_mode, double eps, OptT cos, OptT sin, int64_t rot, OptT pos,
-            int64_t pos_offset, OptT q_out, Tensor err) {
+// -> the rotated q rows (q_out when given), undefined without q heads
+OptT kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, int64_t row0_host, int64_t hq, bool gated,
+                OptT q_norm, OptT k_norm, int64_t norm_mode, double eps, OptT cos, OptT sin, int64_t rot, OptT pos,
+                int64_t pos_offset, OptT q_out) {
   const Cache c(pool, std::move(pages), "kv4.append");
   const int64_t R = (int64_t)c.pages.size();
   need(src, at::kBFloat16, c.pool, "src");
-  need(err, at::kInt, c.pool, "err");
   const int64_t qw = hq * c.hd * (gated ? 2 : 1);
   TORCH_CHECK(src.dim() == 2 && src.stride(1) == 1 && src.size(1) >= qw + 2 * c.hkv * c.hd && hq >= 0 && hq <= 65535,
               "kv4.append: rows [*, q heads | k heads | v heads]");
@@ -140,8 +144,9 @@ void kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
   if (rot > 0 && !pos.has_value() && !row0.has_value())
     TORCH_CHECK((pos_offset < 0 ? row0_host : pos_offset) + T <= a.table_rows,
                 "kv4.append: positions past the RoPE tables' ", std::to_string(a.table_rows));
+  if (hq == 0) q_out = c10::nullopt;
   if (hq > 0) {
-    TORCH_CHECK(q_out.has_value(), "kv4.append: q_out");
+    if (!q_out.has_value()) q_out = at::empty({src.size(0), hq, c.hd}, src.options());
     need(*q_out, at::kBFloat16, c.pool, "q_out");
     TORCH_CHECK(q_out->dim() == 3 && q_out->size(0) == src.size(0) && q_out->size(1) == hq && q_out->size(2) == c.hd &&
                     q_out->stride(2) == 1 && q_out->stride(0) % 8 == 0 && q_out->stride(1) % 8 == 0 && aligned(*q_out),
@@ -151,7 +156,7 @@ void kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
     a.q_out_head = q_out->stride(1);
   }
   TORCH_CHECK(src.size(0) * (hq + 2 * c.hkv) < (1ll << 31), "kv4.append: too many rows");
-  if (T == 0) return;
+  if (T == 0) return q_out;
   a.src = bf(src);
   a.src_row = src.stride(0);
   a.T = (int)T;
@@ -161,8 +166,8 @@ void kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
   a.norm_mode = (int)norm_mode;
   a.eps = eps;
   a.rot = (int)rot;
-  a.err = err.data_ptr<int>();
   c.on_gpu("kv4.append");
+  a.err = c.err();
   c10::cuda::CUDAGuard guard(c.pool.device());
   for (int64_t r0 = 0; r0 < R; r0 += rf::kKv4Seqs) {
     const int n = (int)std::min<int64_t>(rf::kKv4Seqs, R - r0);
@@ -170,35 +175,42 @@ void kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
     rf::kv4_append(a, (int)r0, n, cur());
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return q_out;
 }
 
-void kv4_read(Tensor pool, std::vector<Tensor> pages, OptT row0, int64_t row0_host, Tensor k, Tensor v, Tensor err) {
+// -> k, v [sequences, kv_heads, n, head_dim], or without the first dim (single)
+std::tuple<Tensor, Tensor> kv4_read(Tensor pool, std::vector<Tensor> pages, OptT row0, int64_t row0_host, int64_t n,
+                                    bool single, OptT k_out, OptT v_out) {
   const Cache c(pool, std::move(pages), "kv4.read");
   const int64_t R = (int64_t)c.pages.size();
-  need(err, at::kInt, c.pool, "err");
+  TORCH_CHECK(k_out.has_value() == v_out.has_value(), "kv4.read: both of k and v, or neither");
+  TORCH_CHECK(n >= 0 && n < (1ll << 31) - 64 && (n / 16 + 2) * c.hkv < (1ll << 31) / rf::kKv4Seqs,
+              "kv4.read: a number of rows from 0 to what a launch takes");
+  TORCH_CHECK(!single || R == 1, "kv4.read: one sequence");
+  const auto opts = c.pool.options().dtype(at::kBFloat16);
+  const int64_t lead = single ? 1 : 0;
+  std::vector<int64_t> shape{R, c.hkv, n, c.hd};
+  if (single) shape.erase(shape.begin());
+  Tensor k = k_out.has_value() ? *k_out : at::empty(shape, opts), v = v_out.has_value() ? *v_out : at::empty(shape, opts);
   for (const Tensor* t : {&k, &v}) {
     need(*t, at::kBFloat16, c.pool, "k / v");
-    TORCH_CHECK(t->dim() == 4 && t->size(0) == R && t->size(1) == c.hkv && t->size(3) == c.hd && t->size(2) == k.size(2),
-                "kv4.read: k and v [sequences, kv_heads, rows, head_dim]");
-    TORCH_CHECK(t->numel() == 0 || (t->stride(3) == 1 && t->stride(2) == c.hd && t->stride(0) % 8 == 0 &&
-                                    t->stride(1) % 8 == 0 && t->stride(0) == k.stride(0) &&
-                                    t->stride(1) == k.stride(1) && aligned(*t)),
+    TORCH_CHECK(t->sizes() == at::IntArrayRef(shape), "kv4.read: k and v [sequences, kv_heads, rows, head_dim]");
+    TORCH_CHECK(t->numel() == 0 || (t->stride(3 - lead) == 1 && t->stride(2 - lead) == c.hd && t->stride(1 - lead) % 8 == 0 &&
+                                    (single || t->stride(0) % 8 == 0) && t->strides() == k.strides() && aligned(*t)),
                 "kv4.read: k and v rows head_dim apart, 16-byte aligned, the same strides");
   }
-  const int64_t n = k.size(2);
-  TORCH_CHECK(n < (1ll << 31) - 64 && (n / 16 + 2) * c.hkv < (1ll << 31) / rf::kKv4Seqs, "kv4.read: too many rows");
   rf::Kv4ReadArgs a{};
-  if (R == 0) return;
+  if (R == 0) return {k, v};
   a.row0 = first_rows(row0, row0_host, c, n, "kv4.read");
-  if (n == 0) return;
+  if (n == 0) return {k, v};
   a.row0_host = (int)row0_host;
   a.n = (int)n;
   a.k = bf(k);
   a.v = bf(v);
-  a.out_seq = k.stride(0);
-  a.out_head = k.stride(1);
-  a.err = err.data_ptr<int>();
+  a.out_seq = single ? 0 : k.stride(0);
+  a.out_head = k.stride(1 - lead);
   c.on_gpu("kv4.read");
+  a.err = c.err();
   c10::cuda::CUDAGuard guard(c.pool.device());
   for (int64_t r0 = 0; r0 < R; r0 += rf::kKv4Seqs) {
     const int m = (int)std::min<int64_t>(rf::kKv4Seqs, R - r0);
@@ -206,20 +218,15 @@ void kv4_read(Tensor pool, std::vector<Tensor> pages, OptT row0, int64_t row0_ho
     rf::kv4_read(a, (int)r0, m, cur());
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {k, v};
 }
 
-int64_t kv4_splits(int64_t rows) { return rf::kv4_splits((int)std::min<int64_t>(rows, std::numeric_limits<int>::max())); }
-
-void kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor pos, double scale, OptT gate, int64_t gate_head,
-               Tensor out, Tensor part_o, Tensor part_ml, Tensor err) {
+Tensor kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor pos, double scale, OptT gate,
+                     int64_t gate_head, OptT out_given) {
   const Cache c(pool, std::move(pages), "kv4.attention");
   const int64_t R = (int64_t)c.pages.size();
   need(q, at::kBFloat16, c.pool, "q");
   need(pos, at::kInt, c.pool, "pos");
-  need(out, at::kBFloat16, c.pool, "out");
-  need(part_o, at::kFloat, c.pool, "part_o");
-  need(part_ml, at::kFloat, c.pool, "part_ml");
-  need(err, at::kInt, c.pool, "err");
   TORCH_CHECK(q.dim() == 3 && q.size(0) == R && q.size(2) == c.hd && q.stride(2) == 1 && q.stride(1) % 8 == 0 &&
                   (R <= 1 || q.stride(0) % 8 == 0) && aligned(q),
               "kv4.attention: q [sequences, q heads, head_dim], 16-byte aligned");
@@ -227,6 +234,8 @@ void kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor pos,
   TORCH_CHECK(hq % c.hkv == 0 && hq / c.hkv >= 1 && hq / c.hkv <= 8, "kv4.attention: 1 to 8 query heads per KV head, not ",
               std::to_string(hq), " over ", std::to_string(c.hkv));
   TORCH_CHECK(pos.dim() == 1 && pos.is_contiguous() && pos.numel() == R, "kv4.attention: one position per sequence");
+  Tensor out = out_given.has_value() ? *out_given : at::empty({R, hq * c.hd}, q.options());
+  need(out, at::kBFloat16, c.pool, "out");
   TORCH_CHECK(out.dim() == 2 && out.size(0) == R && out.size(1) == hq * c.hd && out.stride(1) == 1 && aligned(out) &&
                   (R <= 1 || out.stride(0) % 8 == 0),
               "kv4.attention: out [sequences, q heads * head_dim], 16-byte aligned");
@@ -241,13 +250,14 @@ void kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor pos,
     a.gate_row = gate->stride(0);
     a.gate_head = gate_head;
   }
-  if (R == 0) return;
+  if (R == 0) return out;
+  c.on_gpu("kv4.attention");
   int64_t most = 1;
   for (int64_t r = 0; r < R; ++r) most = std::max(most, c.rows(r));
-  const int64_t S = kv4_splits(most);
-  TORCH_CHECK(part_o.is_contiguous() && part_o.numel() >= R * S * hq * c.hd && part_ml.is_contiguous() &&
-                  part_ml.numel() >= R * S * hq * 2 && aligned(part_o) && aligned(part_ml),
-              "kv4.attention: workspace");
+  const int64_t S = rf::kv4_splits((int)most);
+  // the splits' outputs, maxima and sums: this call's own, so calls on other streams and graphs share nothing
+  Tensor parts;
+  if (S > 1) parts = at::empty({R * S * hq * (c.hd + 2)}, q.options().dtype(at::kFloat));
   a.q = bf(q);
   a.q_row = q.stride(0);
   a.q_head = q.stride(1);
@@ -257,10 +267,9 @@ void kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor pos,
   a.out = bf(out);
   a.out_row = out.stride(0);
   a.splits = (int)S;
-  a.part_o = part_o.data_ptr<float>();
-  a.part_ml = part_ml.data_ptr<float>();
-  a.err = err.data_ptr<int>();
-  c.on_gpu("kv4.attention");
+  a.part_o = S > 1 ? parts.data_ptr<float>() : nullptr;
+  a.part_ml = S > 1 ? a.part_o + R * S * hq * c.hd : nullptr;
+  a.err = c.err();
   c10::cuda::CUDAGuard guard(c.pool.device());
   for (int64_t r0 = 0; r0 < R; r0 += rf::kKv4Seqs) {
     const int n = (int)std::min<int64_t>(rf::kKv4Seqs, R - r0);
@@ -268,6 +277,7 @@ void kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor pos,
     rf::kv4_attention(a, (int)r0, n, cur());
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
 }
 
 }  // namespace
@@ -275,6 +285,5 @@ void kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor pos,
 void register_kv4(pybind11::module_& m) {
   m.def("kv4_append", &kv4_append);
   m.def("kv4_read", &kv4_read);
-  m.def("kv4_splits", &kv4_splits);
   m.def("kv4_attention", &kv4_attention);
 }

@@ -283,6 +283,7 @@ template <int HD>
 __global__ void __launch_bounds__(256)
     kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows, int down) {
   constexpr int PER = HD / 32;
+  allow_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = a.hq + 2 * a.c.hkv;
   const int n = down ? blockIdx.x : blockIdx.x * 8 + warp;   // row of this launch

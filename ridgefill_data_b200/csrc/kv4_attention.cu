@@ -96,10 +96,6 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t* w) {
   }
 }
 
-// The next kernel of the stream may start before this one ends (its first act is to wait for it) / that wait.
-__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // out = o / sum * sigmoid(gate) for 4 dims of a head. A sum of -inf (or NaN) tells of a visible row with non-finite
 // values; 0 of no row at all.
 __device__ __forceinline__ void finish(const Kv4AttnArgs& a, int r, int col, int h, int e, float4 o, float sum) {
@@ -416,14 +412,15 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.hq / a.c.hkv;
   allow_next();
-  QueryLoad<HD> loading;                           // in flight while the position and the page ids are fetched
-  loading.load(a, a.q + (long)r * a.q_row + (long)g * G * a.q_head, G, warp, lane);
+  // before the previous kernel (this step's append, usually) has ended: positions and page ids alone, which it does not
+  // write; everything it may have written, and every store, after the wait
   const int p = a.pos[r];
   if (p < 0 || p >= a.c.rows[sq]) {
-    if (p >= 0 && s == 0 && g == 0 && threadIdx.x == 0) record_error(a.err, kErrBadIndex);
-    if (s == 0)
-      for (int x = threadIdx.x; x < G * HD / 4; x += kWarps * 32)
-        kv4_store<4>(a.out + (long)r * a.out_row + g * G * HD + 4 * x, {0.f, 0.f, 0.f, 0.f});
+    if (s > 0) return;
+    wait_previous();
+    if (p >= 0 && g == 0 && threadIdx.x == 0) record_error(a.err, kErrBadIndex);
+    for (int x = threadIdx.x; x < G * HD / 4; x += kWarps * 32)
+      kv4_store<4>(a.out + (long)r * a.out_row + g * G * HD + 4 * x, {0.f, 0.f, 0.f, 0.f});
     return;
   }
   const int keys = split_keys(p), start = s * keys;
@@ -463,10 +460,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
   if (lane < ST) mbar_init(bar + lane, NB);
   fence_barrier_init();
   __syncwarp();
-  if (lane < ST * NB && mine - lane % NB < blocks) {
-    if (mine < blocks) id = __ldg(table + page);
-    issue();
-  }
+  if (lane < ST * NB && mine < blocks) id = __ldg(table + page);
+  wait_previous();
+  QueryLoad<HD> loading;
+  loading.load(a, a.q + (long)r * a.q_row + (long)g * G * a.q_head, G, warp, lane);
+  if (lane < ST * NB && mine - lane % NB < blocks) issue();
   __syncwarp();
   const uint2 sums = loading.prepare(query, a.scale_log2, warp, lane);
   Warp<HD> w;
@@ -545,6 +543,7 @@ __global__ void __launch_bounds__(HD / 4 * kJoin) kv4_combine_kernel(const __gri
   const int h = blockIdx.x, sq = blockIdx.y, r = r0 + sq;
   const int x = threadIdx.x % (HD / 4), y = threadIdx.x / (HD / 4);
   wait_previous();
+  allow_next();
   const int p = a.pos[r];
   if (p >= a.c.rows[sq] || p < split_keys(0)) return;   // no row, or one split: written by it
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -596,18 +595,23 @@ void launch(const Kv4AttnArgs& a, int r0, int seqs, cudaStream_t stream) {
   once([] {
     cudaFuncSetAttribute(kv4_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM);
   });
-  kv4_attn_kernel<HD><<<dim3(a.splits, a.c.hkv, seqs), kWarps * 32, Cfg<HD>::SMEM, stream>>>(a, r0);
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.splits, a.c.hkv, seqs);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = Cfg<HD>::SMEM;
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kv4_attn_kernel<HD>, a, r0) != cudaSuccess)
+    throw std::runtime_error("kv4_attention: launch failed");
   count_launch();
   if (a.splits > 1) {
-    cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.hq, seqs);
     cfg.blockDim = dim3(HD / 4 * kJoin);
-    cfg.stream = stream;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
+    cfg.dynamicSmemBytes = 0;
     if (cudaLaunchKernelEx(&cfg, kv4_combine_kernel<HD>, a, r0) != cudaSuccess)
       throw std::runtime_error("kv4_attention: launch of the join failed");
     count_launch();

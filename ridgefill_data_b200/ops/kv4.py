@@ -48,16 +48,12 @@ def pool(pages, n_kv, page_size, head_dim, device="cuda"):
 
 
 def _tables(pages):
-    return [pages] if torch.is_tensor(pages) else list(pages)
+    return [pages] if torch.is_tensor(pages) else pages
 
 
 def _row0(row0):
     """(device rows, host row): a tensor of first rows, or one host integer."""
     return (row0, 0) if torch.is_tensor(row0) else (None, int(row0))
-
-
-def _err(pool):
-    return ext().error_word(pool.device.index or 0) if pool.is_cuda else torch.zeros(1, dtype=torch.int32)
 
 
 def append(src, pool, pages, row0, q_heads=0, gated=False, q_norm=None, k_norm=None, norm_mode=-1, eps=1e-6,
@@ -70,28 +66,18 @@ def append(src, pool, pages, row0, q_heads=0, gated=False, q_norm=None, k_norm=N
     sin) bf16 [positions, rot / 2]. Roundings as the bf16 model's; the norm's sum and root in 64 bits.
     Returns the rotated q rows [R * T, q_heads, head_dim] (q_out when given, with any row and head pitch), or None."""
     cos, sin = tables if tables is not None and rot else (None, None)
-    if q_heads and q_out is None:
-        q_out = torch.empty(src.shape[0], q_heads, (pool.shape[-1] - 32) // 20, dtype=BF16, device=src.device)
     dev, host = _row0(row0)
-    ext().kv4_append(src, pool, _tables(pages), dev, host, int(q_heads), bool(gated), q_norm, k_norm, int(norm_mode),
-                     float(eps), cos, sin, int(rot), pos, int(pos_offset), q_out if q_heads else None, _err(pool))
-    return q_out if q_heads else None
+    return ext().kv4_append(src, pool, _tables(pages), dev, host, q_heads, gated, q_norm, k_norm, norm_mode, eps, cos, sin,
+                            rot, pos, pos_offset, q_out)
 
 
 def read(pool, pages, n, row0=0, out=None):
     """(k, v) bf16 [R, kv_heads, n, head_dim]: cache rows row0[r] .. row0[r] + n of every sequence (row0 as in append; a
     skipped sequence reads zeros); without the first dim when `pages` is one table instead of a list. out: (k, v) to
     write into, of equal strides."""
-    single = torch.is_tensor(pages)
-    pages = _tables(pages)
-    if out is None:
-        shape = (len(pages), pool.shape[1], int(n), (pool.shape[-1] - 32) // 20)
-        k, v = (torch.empty(shape, dtype=BF16, device=pool.device) for _ in range(2))
-    else:
-        k, v = (t.unsqueeze(0) for t in out) if single else out
+    k, v = out if out is not None else (None, None)
     dev, host = _row0(row0)
-    ext().kv4_read(pool, pages, dev, host, k, v, _err(pool))
-    return (k[0], v[0]) if single else (k, v)
+    return ext().kv4_read(pool, _tables(pages), dev, host, n, torch.is_tensor(pages), k, v)
 
 
 def attention(q, pool, pages, pos, scale, out=None, gate=None, gate_head=0):
@@ -99,13 +85,4 @@ def attention(q, pool, pages, pos, scale, out=None, gate=None, gate_head=0):
     of its pages (pos int32 [R] on the device; negative: no rows, the output is zero). gate: a [R, *] view whose head h
     starts at column h * gate_head (o * sigmoid(gate)). Returns out [R, q_heads * head_dim] bf16. The keys are split
     by pos alone: a sequence gets the same bits alone or batched, whatever pages hold it."""
-    pages = _tables(pages)
-    R, hq, hd = q.shape
-    most = max((t.numel() for t in pages), default=0) * pool.shape[2] * BLOCK
-    S = ext().kv4_splits(most)
-    part_o = torch.empty(R * S * hq * hd, dtype=torch.float32, device=q.device)
-    part_ml = torch.empty(R * S * hq * 2, dtype=torch.float32, device=q.device)
-    if out is None:
-        out = torch.empty(R, hq * hd, dtype=BF16, device=q.device)
-    ext().kv4_attention(q, pool, pages, pos, float(scale), gate, int(gate_head), out, part_o, part_ml, _err(pool))
-    return out
+    return ext().kv4_attention(q, pool, _tables(pages), pos, scale, gate, gate_head, out)
