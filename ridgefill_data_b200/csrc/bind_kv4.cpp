@@ -20,6 +20,7 @@ using OptT = c10::optional<Tensor>;
 
 cudaStream_t cur() { return at::cuda::getCurrentCUDAStream().stream(); }
 __nv_bfloat16* bf(const Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
+bool small(int64_t stride) { return stride >= 0 && stride < (1ll << 31); }
 bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 // Numbers reach a message as std::to_string: streaming one faults where the compiler's libstdc++ is not torch's.
@@ -101,7 +102,8 @@ OptT kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
   const int64_t qw = hq * c.hd * (gated ? 2 : 1);
   TORCH_CHECK(src.dim() == 2 && src.stride(1) == 1 && src.size(1) >= qw + 2 * c.hkv * c.hd && hq >= 0 && hq <= 65535,
               "kv4.append: rows [*, q heads | k heads | v heads]");
-  TORCH_CHECK(aligned(src) && (src.size(0) <= 1 || src.stride(0) % 8 == 0), "kv4.append: 16-byte aligned rows");
+  TORCH_CHECK(aligned(src) && (src.size(0) <= 1 || src.stride(0) % 8 == 0) && small(src.stride(0)),
+              "kv4.append: 16-byte aligned rows");
   TORCH_CHECK(R > 0 && src.size(0) % R == 0, "kv4.append: the same number of rows for every sequence");
   const int64_t T = src.size(0) / R;
   TORCH_CHECK(T < (1 << 30), "kv4.append: too many rows");
@@ -149,16 +151,16 @@ OptT kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
     if (!q_out.has_value()) q_out = at::empty({src.size(0), hq, c.hd}, src.options());
     need(*q_out, at::kBFloat16, c.pool, "q_out");
     TORCH_CHECK(q_out->dim() == 3 && q_out->size(0) == src.size(0) && q_out->size(1) == hq && q_out->size(2) == c.hd &&
-                    q_out->stride(2) == 1 && q_out->stride(0) % 8 == 0 && q_out->stride(1) % 8 == 0 && aligned(*q_out),
+                    q_out->stride(2) == 1 && small(q_out->stride(0)) && small(q_out->stride(1)) && q_out->stride(0) % 8 == 0 && q_out->stride(1) % 8 == 0 && aligned(*q_out),
                 "kv4.append: q_out [rows, q heads, head_dim], 16-byte aligned");
     a.q_out = bf(*q_out);
-    a.q_out_row = q_out->stride(0);
-    a.q_out_head = q_out->stride(1);
+    a.q_out_row = (int)q_out->stride(0);
+    a.q_out_head = (int)q_out->stride(1);
   }
   TORCH_CHECK(src.size(0) * (hq + 2 * c.hkv) < (1ll << 31), "kv4.append: too many rows");
   if (T == 0) return q_out;
   a.src = bf(src);
-  a.src_row = src.stride(0);
+  a.src_row = (int)src.stride(0);
   a.T = (int)T;
   a.hq = (int)hq;
   a.q_stride = c.hd * (gated ? 2 : 1);

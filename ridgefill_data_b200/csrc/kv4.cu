@@ -2,7 +2,7 @@
 //
 // kv4_append_kernel  a warp per row and head (q | k | v), a lane holding hd / 32 consecutive values: head norm and rotation
 //                    (q, k), then q goes out in bf16 and k / v rows are quantised into their block.
-// kv4_append_q_kernel, kv4_append_kv_kernel  the same for many rows (below).
+// kv4_append_rows_kernel  the same for many rows (below).
 // kv4_read_kernel    one warp per block of 16 rows: the block to shared memory in 16-byte pieces, then row by row the values
 //                    the codes stand for, rounded once to bf16, a whole row per store instruction.
 //
@@ -290,9 +290,9 @@ __global__ void __launch_bounds__(256)
   const int head = down ? blockIdx.y * 8 + warp : blockIdx.y, kh = head - a.hq;
   if (n >= rows || head >= heads) return;
   const int sq = a.T == 1 ? n : n < a.T ? 0 : n / a.T, t = n - sq * a.T;
-  const long src_row = (long)r0 * a.T + n;
+  const int src_row = r0 * a.T + n;
   Row<PER> v, w;
-  v.load(a.src + src_row * a.src_row + lane * PER + (kh < 0 ? head * a.q_stride : a.k_col + kh * HD));
+  v.load(a.src + (long)src_row * a.src_row + lane * PER + (kh < 0 ? head * a.q_stride : a.k_col + kh * HD));
   const bool normed = kh < a.c.hkv && a.norm_mode >= 0;
   if (normed) w.load((kh < 0 ? a.q_norm : a.k_norm) + lane * PER);
   const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(256)
     if (!ok)
 #pragma unroll
       for (int j = 0; j < PER / 2; ++j) v.w[j] = 0;
-    v.store(a.q_out + src_row * a.q_out_row + (long)head * a.q_out_head + lane * PER);
+    v.store(a.q_out + (long)src_row * a.q_out_row + (long)head * a.q_out_head + lane * PER);
   } else if (kh < a.c.hkv) {
     put_row<HD, false>(v, block, row & 15, lane);
   } else {
@@ -333,21 +333,25 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Many rows: the queries and the cached rows go their own ways.
+// Many rows: the queries and the cached rows go their own ways in one launch (kv4_append_rows_kernel).
 //
-// kv4_append_q_kernel   a lane holds 8 values (16 bytes), so a warp's loads and stores are whole sectors whatever the head
+// query_rows            a lane holds 8 values (16 bytes), so a warp's loads and stores are whole sectors whatever the head
 //                       size: 256 / hd heads of a row at a time, two times. The rotation's half is whole lanes (rot / 2 a
 //                       multiple of 8).
-// kv4_append_kv_kernel  a CTA per block of 16 cache rows and 512 / hd heads of K or of V, a warp two rows: a lane holds 16 values (half a
-//                       group), hd / 16 lanes a head, so what is done once a head or a group is done for all its heads at
-//                       once; the block's bytes are put together in shared memory and leave as 16-byte pieces (row by row
+// cache_block           a CTA per block of 16 cache rows and 512 / hd heads of K or of V, a warp two rows: a lane holds 16
+//                       values (half a group), hd / 16 lanes a head, so what is done once a head or a group is done for all
+//                       its heads at once; the block's bytes are put together in shared memory and leave as 16-byte pieces (row by row
 //                       they would be 24 partial sectors a row and head). A block that is only partly appended is written
 //                       in place, row by row. The rotation's half is whole lanes (rot / 2 a multiple of 16).
+
+// kept out of line: the common cases branch past it
+__device__ __noinline__ int divide(int a, int b) { return a / b; }
+
 struct Place {
   int row, p;   // cache row (negative: the sequence is skipped), rotary position
   bool ok;
 };
-__device__ __forceinline__ Place place(const Kv4AppendArgs& a, int first, int sq, int t, long src_row) {
+__device__ __forceinline__ Place place(const Kv4AppendArgs& a, int first, int sq, int t, int src_row) {
   Place f;
   const unsigned row = (unsigned)first + t;   // below 2^32: first < 2^31, t < 2^30
   f.p = a.pos != nullptr ? __ldg(a.pos + src_row) : a.pos_offset >= 0 ? a.pos_offset + t : (int)row;
@@ -356,66 +360,74 @@ __device__ __forceinline__ Place place(const Kv4AppendArgs& a, int first, int sq
   return f;
 }
 
+// 16 rows of 2 x 256 / hd query heads: a warp two rows, their loads in flight together.
 template <int HD, int MODE, bool TURN>
-__global__ void __launch_bounds__(256) kv4_append_q_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows) {
+__device__ __forceinline__ void query_rows(const Kv4AppendArgs& a, int r0, int rows, int x, int set) {
   constexpr int LANES = HD / 8, HEADS = 32 / LANES;
   const int lane = threadIdx.x & 31, j = lane % LANES;
-  const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (n >= rows) return;
-  const int head = blockIdx.y * 2 * HEADS + lane / LANES;   // and HEADS further
-  const long src_row = (long)r0 * a.T + n;
-  const __nv_bfloat16* src = a.src + src_row * a.src_row + 8 * j;
-  Row<8> v[2], w;
+  const int n0 = x * 16 + (threadIdx.x >> 5);
+  if (n0 >= rows) return;
+  const int head = set * 2 * HEADS + lane / LANES;   // and HEADS further
   const bool there[2] = {head < a.hq, head + HEADS < a.hq};
+  Row<8> v[2][2], w;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) v[x].load(src + (there[x] ? (head + x * HEADS) * a.q_stride : 0));
+  for (int u = 0; u < 2; ++u) {
+    const int src_row = r0 * a.T + min(n0 + 8 * u, rows - 1);
+    const __nv_bfloat16* src = a.src + (long)src_row * a.src_row + 8 * j;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) v[u][y].load(src + (there[y] ? (head + y * HEADS) * a.q_stride : 0));
+  }
   if constexpr (MODE >= 0) w.load(a.q_norm + 8 * j);
-  int sq = 0, t = n;
-  if (t >= a.T) sq = n / a.T, t = n - sq * a.T;
-  const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
-  const Place f = place(a, first, sq, t, src_row);
+  const int h = a.rot / 2, i0 = 8 * j;
+  const bool low = i0 < h;
   Turn<8> turn;
-  if constexpr (TURN) {
-    const int h = a.rot / 2, i0 = 8 * j;
-    const bool low = i0 < h;
-    turn.in = i0 < a.rot;
-    turn.from = !turn.in ? lane : low ? lane + h / 8 : lane - h / 8;
-    const long entry = f.ok && turn.in ? (long)f.p * h + (low ? i0 : i0 - h) : 0;
-    turn.c.load(a.cos + entry);
-    turn.s.load(a.sin + entry);
+  turn.in = i0 < a.rot;
+  turn.from = !turn.in ? lane : low ? lane + h / 8 : lane - h / 8;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) turn.s.w[x] ^= low ? 0x80008000u : 0u;
-  }
-  if constexpr (MODE >= 0) {
+  for (int u = 0; u < 2; ++u) {
+    const int n = n0 + 8 * u;
+    if (n >= rows) break;
+    const int src_row = r0 * a.T + n;
+    int sq = 0, t = n;
+    if (t >= a.T) sq = divide(n, a.T), t = n - sq * a.T;
+    const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
+    const Place f = place(a, first, sq, t, src_row);
+    if constexpr (TURN) {
+      const long entry = f.ok && turn.in ? (long)f.p * h + (low ? i0 : i0 - h) : 0;
+      turn.c.load(a.cos + entry);
+      turn.s.load(a.sin + entry);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      // the sums of the hd / 32 values that a lane holds when a warp takes one head, added across in that order too: the
-      // same bits as there
-      constexpr int PARTS = 256 / HD, PER = HD / 32;
-      float ss[PARTS];
-#pragma unroll
-      for (int y = 0; y < PARTS; ++y) {
-        ss[y] = 0.f;
-#pragma unroll
-        for (int z = 0; z < PER; ++z) ss[y] = fmaf(v[x].get(y * PER + z), v[x].get(y * PER + z), ss[y]);
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) ss[y] += __shfl_xor_sync(kFull, ss[y], o);
-      }
-#pragma unroll
-      for (int o = PARTS / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int y = 0; y < o; ++y) ss[y] += ss[y + o];
-      const float inv = rsqrtf(ss[0] / (float)HD + (float)a.eps);
-#pragma unroll
-      for (int y = 0; y < 4; ++y) v[x].w[y] = query_pair(inv, v[x].w[y], w.w[y], MODE);
+      for (int z = 0; z < 4; ++z) turn.s.w[z] ^= low ? 0x80008000u : 0u;
     }
-  }
-  __nv_bfloat16* dst = a.q_out + src_row * a.q_out_row + 8 * j;
+    __nv_bfloat16* dst = a.q_out + (long)src_row * a.q_out_row + 8 * j;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    if constexpr (TURN) turn.apply(v[x]);
-    if (!f.ok) v[x].w[0] = v[x].w[1] = v[x].w[2] = v[x].w[3] = 0;
-    if (there[x]) v[x].store(dst + (long)(head + x * HEADS) * a.q_out_head);
+    for (int y = 0; y < 2; ++y) {
+      Row<8>& q = v[u][y];
+      if constexpr (MODE >= 0) {
+        // the sums of the hd / 32 values that a lane holds when a warp takes one head, added across in that order too:
+        // the same bits as there
+        constexpr int PARTS = 256 / HD, PER = HD / 32;
+        float ss[PARTS];
+#pragma unroll
+        for (int y = 0; y < PARTS; ++y) {
+          ss[y] = 0.f;
+#pragma unroll
+          for (int z = 0; z < PER; ++z) ss[y] = fmaf(q.get(y * PER + z), q.get(y * PER + z), ss[y]);
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) ss[y] += __shfl_xor_sync(kFull, ss[y], o);
+        }
+#pragma unroll
+        for (int o = PARTS / 2; o > 0; o >>= 1)
+#pragma unroll
+          for (int y = 0; y < o; ++y) ss[y] += ss[y + o];
+        const float inv = rsqrtf(ss[0] / (float)HD + (float)a.eps);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) q.w[y] = query_pair(inv, q.w[y], w.w[y], MODE);
+      }
+      if constexpr (TURN) turn.apply(q);
+      if (!f.ok) q.w[0] = q.w[1] = q.w[2] = q.w[3] = 0;
+      if (there[y]) q.store(dst + (long)(head + y * HEADS) * a.q_out_head);
+    }
   }
 }
 
@@ -492,15 +504,11 @@ __device__ __forceinline__ void cache_row(uint32_t (&v)[8], const Kv4AppendArgs&
   if (j == 0) block[(IS_V ? L::VE : L::KE) + r] = (uint8_t)(bad ? kKv4Mark : e + 127);
 }
 
-// kept out of line: the common page sizes are powers of two and branch past it
-__device__ __noinline__ int divide(int a, int b) { return a / b; }
-
 template <int HD, bool IS_V, int MODE, bool TURN>
-__device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs& a, int r0, int set) {
+__device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs& a, int r0, int sq, int x, int set) {
   using L = Kv4L<HD>;
   constexpr int LANES = HD / 16, HEADS = 32 / LANES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sq = blockIdx.z, x = blockIdx.x;
   const int head = set * HEADS + lane / LANES;
   const bool there = head < a.c.hkv;
   const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
@@ -516,8 +524,8 @@ __device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs&
   for (int u = 0; u < 2; ++u) {
     const int t = t0 + warp + 8 * u;
     const bool mine = t >= 0 && t < a.T;
-    const long src_row = (long)(r0 + sq) * a.T + (mine ? t : 0);
-    const uint4* at = reinterpret_cast<const uint4*>(src + src_row * a.src_row);
+    const int src_row = (r0 + sq) * a.T + (mine ? t : 0);
+    const uint4* at = reinterpret_cast<const uint4*>(src + (long)src_row * a.src_row);
     const uint4 y = __ldg(at), z = __ldg(at + 1);
     v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w, v[u][4] = z.x, v[u][5] = z.y, v[u][6] = z.z, v[u][7] = z.w;
     f[u] = place(a, first, sq, t, src_row);
@@ -560,13 +568,31 @@ __device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs&
   }
 }
 
+// Queries (bound by their bytes) and cached rows (bound by their arithmetic) of one call side by side: CTA i takes a block of
+// the cache when i kv / (q + kv) reaches its next whole number, else query rows.
+struct AppendPlan {
+  int q_rows, q_sets;          // CTAs of the queries: 16-row pieces, sets of heads
+  int spans, kv_sets, seqs;    // of the cache: blocks of a sequence, 2 x sets of KV heads, sequences
+};
+
 template <int HD, int MODE, bool TURN>
-__global__ void __launch_bounds__(256, MODE == 1 ? 2 : 3) kv4_append_kv_kernel(const __grid_constant__ Kv4AppendArgs a, int r0) {
+__global__ void __launch_bounds__(256, 4)
+    kv4_append_rows_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows, const AppendPlan plan) {
   __shared__ __align__(16) uint8_t image[512 / HD * Kv4L<HD>::BYTES];
-  if (blockIdx.y & 1)
-    cache_block<HD, true, -1, false>(image, a, r0, blockIdx.y / 2);
-  else
-    cache_block<HD, false, MODE, TURN>(image, a, r0, blockIdx.y / 2);
+  allow_next();
+  const unsigned kv = (unsigned)plan.spans * plan.kv_sets * plan.seqs, all = gridDim.x, i = blockIdx.x;
+  const unsigned at = (unsigned)((unsigned long long)i * kv / all);
+  if ((unsigned)((unsigned long long)(i + 1) * kv / all) > at) {
+    // kv sets of one block side by side: they share the rows of the source
+    const int set = at % plan.kv_sets, x = at / plan.kv_sets % plan.spans, sq = at / plan.kv_sets / plan.spans;
+    if (set & 1)
+      cache_block<HD, true, -1, false>(image, a, r0, sq, x, set / 2);
+    else
+      cache_block<HD, false, MODE, TURN>(image, a, r0, sq, x, set / 2);
+  } else {
+    const int q = i - at;
+    query_rows<HD, MODE, TURN>(a, r0, rows, q / plan.q_sets, q % plan.q_sets);
+  }
 }
 
 constexpr int kReadWarps = 4;
@@ -644,16 +670,17 @@ __global__ void __launch_bounds__(kReadWarps * 32) kv4_read_kernel(const __grid_
 
 template <int HD, int MODE, bool TURN>
 void launch_rows(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) {
+  constexpr int HEADS = 512 / HD;
   const int rows = seqs * a.T;
-  if (a.hq > 0) {
-    kv4_append_q_kernel<HD, MODE, TURN>
-        <<<dim3((rows + 7) / 8, (a.hq + 512 / HD - 1) / (512 / HD)), 256, 0, stream>>>(a, r0, rows);
-    count_launch();
-  }
+  AppendPlan plan{};
+  plan.q_rows = (rows + 15) / 16;
+  plan.q_sets = (a.hq + HEADS - 1) / HEADS;
   // blocks that T rows can touch: known exactly for a host row, else one more
-  const int spans = a.row0 == nullptr ? (int)(((long)a.row0_host + a.T - 1) / 16 - a.row0_host / 16 + 1) : (a.T + 14) / 16 + 1;
-  kv4_append_kv_kernel<HD, MODE, TURN>
-      <<<dim3(spans, 2 * ((a.c.hkv + 512 / HD - 1) / (512 / HD)), seqs), 256, 0, stream>>>(a, r0);
+  plan.spans = a.row0 == nullptr ? (int)(((long)a.row0_host + a.T - 1) / 16 - a.row0_host / 16 + 1) : (a.T + 14) / 16 + 1;
+  plan.kv_sets = 2 * ((a.c.hkv + HEADS - 1) / HEADS);
+  plan.seqs = seqs;
+  const unsigned grid = (unsigned)plan.q_rows * plan.q_sets + (unsigned)plan.spans * plan.kv_sets * seqs;
+  kv4_append_rows_kernel<HD, MODE, TURN><<<grid, 256, 0, stream>>>(a, r0, rows, plan);
   count_launch();
 }
 

@@ -19,7 +19,7 @@ struct Kv4Pages {
 struct Kv4AppendArgs {
   Kv4Pages c;
   const __nv_bfloat16* src;       // [R * T, *] projected rows: q heads (each [q | gate] when gated) | k heads | v heads
-  long src_row;
+  int src_row;
   int T;                          // rows a sequence
   int hq, q_stride;               // q heads (0: no q), elements between their starts
   int k_col;                      // column of the first k head (the v heads follow the k heads)
@@ -35,7 +35,7 @@ struct Kv4AppendArgs {
   const int* pos;                 // [R * T] rotary positions, or nullptr: pos_offset + the row's index (pos_offset >= 0),
   int pos_offset;                 // or the cache row (pos_offset < 0)
   __nv_bfloat16* q_out;           // rotated q rows
-  long q_out_row, q_out_head;
+  int q_out_row, q_out_head;
   int page_shift;                 // log2 of the page size, -1 when it is no power of two (set by the launch)
   int* err;
 };
