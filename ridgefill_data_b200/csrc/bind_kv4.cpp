@@ -256,7 +256,7 @@ Tensor kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor po
   c.on_gpu("kv4.attention");
   int64_t most = 1;
   for (int64_t r = 0; r < R; ++r) most = std::max(most, c.rows(r));
-  const int64_t S = rf::kv4_splits((int)most);
+  const int64_t S = rf::kv4_splits((int)most, c.hd, c.hkv);
   // the splits' outputs, maxima and sums: this call's own, so calls on other streams and graphs share nothing
   Tensor parts;
   if (S > 1) parts = at::empty({R * S * hq * (c.hd + 2)}, q.options().dtype(at::kFloat));
@@ -269,6 +269,8 @@ Tensor kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor po
   a.out = bf(out);
   a.out_row = out.stride(0);
   a.splits = (int)S;
+  a.most = rf::kv4_most_splits(c.hd, c.hkv);
+  a.most = rf::kv4_most_splits(c.hd, c.hkv);
   a.part_o = S > 1 ? parts.data_ptr<float>() : nullptr;
   a.part_ml = S > 1 ? a.part_o + R * S * hq * c.hd : nullptr;
   a.err = c.err();

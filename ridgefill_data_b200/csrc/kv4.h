@@ -53,7 +53,7 @@ struct Kv4ReadArgs {
 };
 void kv4_read(const Kv4ReadArgs& a, int r0, int seqs, cudaStream_t stream);
 
-constexpr int kKv4Splits = 64;    // key splits per (sequence, KV head), at most
+constexpr int kKv4Splits = 128;   // key splits per (sequence, KV head), at most
 struct Kv4AttnArgs {
   Kv4Pages c;
   const __nv_bfloat16* q;         // [R, hq, hd] rotated query rows
@@ -66,11 +66,13 @@ struct Kv4AttnArgs {
   __nv_bfloat16* out;             // [R, hq * hd]
   long out_row;
   int splits;                     // splits the longest sequence's rows can need (the launch's grid)
+  int most;                       // splits a sequence may have (kv4_most_splits)
   float* part_o;                  // [R, hkv, splits, G, hd]
   float* part_ml;                 // [R, hkv, splits, G, 2]
   int* err;
 };
-int kv4_splits(int rows);         // splits that a sequence of `rows` cache rows needs at most
+int kv4_most_splits(int hd, int hkv);
+int kv4_splits(int rows, int hd, int hkv);   // splits that a sequence of `rows` cache rows needs at most
 void kv4_attention(const Kv4AttnArgs& a, int r0, int seqs, cudaStream_t stream);
 
 }  // namespace rf

@@ -31,8 +31,11 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 4;
 constexpr float kLow = -1e30f;   // below every score: exp2 of a difference to it is 0, never NaN
 
-constexpr int kUnit = 512;       // keys of a split, up to kKv4Splits of them; then a multiple
-__host__ __device__ constexpr int split_keys(int p) { return kUnit * (p / (kUnit * kKv4Splits) + 1); }
+constexpr int kUnit = 512;         // keys of a split, at least
+constexpr int kTile = 128;         // and a multiple of this: every warp whole runs of blocks
+
+// keys of a split of rows 0 .. p when there may be `splits` of them
+__host__ __device__ inline int split_keys(int p, int splits) { return max(kUnit, kTile * (p / (kTile * splits) + 1)); }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -423,7 +426,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
       kv4_store<4>(a.out + (long)r * a.out_row + g * G * HD + 4 * x, {0.f, 0.f, 0.f, 0.f});
     return;
   }
-  const int keys = split_keys(p), start = s * keys;
+  const int keys = split_keys(p, a.most), start = s * keys;
   if (start > p) return;
   const int end = min(start + keys, p + 1);
   // the split's blocks in runs of NB: runs warp, warp + 4, ... Lane x of the first ST NB drives slot x of the ring: its
@@ -545,10 +548,10 @@ __global__ void __launch_bounds__(HD / 4 * kJoin) kv4_combine_kernel(const __gri
   wait_previous();
   allow_next();
   const int p = a.pos[r];
-  if (p >= a.c.rows[sq] || p < split_keys(0)) return;   // no row, or one split: written by it
+  if (p >= a.c.rows[sq] || p < kUnit) return;   // no row, or one split: written by it
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float S = 0.f;
-  const int ns = p / split_keys(p) + 1;
+  const int ns = p / split_keys(p, a.most) + 1;
   const long base = ((long)r * a.c.hkv + h / G) * a.splits * G + h % G;
   // every warp finds the largest maximum and the sum; the split's weight for all from the first
   const int lane = threadIdx.x & 31;
@@ -620,7 +623,18 @@ void launch(const Kv4AttnArgs& a, int r0, int seqs, cudaStream_t stream) {
 
 }  // namespace
 
-int kv4_splits(int rows) { return rows <= 0 ? 1 : std::min(kKv4Splits, (rows - 1) / kUnit + 1); }
+// As many splits as the KV heads of one long sequence need to fill the GPU once (148 SMs of Cfg::CTAS each), in steps of 32
+// from 64 to kKv4Splits: by the model's shape alone, so the split of a sequence does not depend on the batch. (One
+// sequence behind 128K rows of 4 heads of 256: 64 splits 47 us, 111 45 us; four behind 128K rows of 8 heads of 128: 64
+// splits 130 us, 74 133 us.)
+int kv4_most_splits(int hd, int hkv) {
+  const int slots = 148 * (hd == 256 ? Cfg<256>::CTAS : hd == 128 ? Cfg<128>::CTAS : Cfg<64>::CTAS);
+  return std::max(64, std::min(kKv4Splits, slots / hkv / 32 * 32));
+}
+
+int kv4_splits(int rows, int hd, int hkv) {
+  return rows <= 0 ? 1 : std::min(kv4_most_splits(hd, hkv), (rows - 1) / kUnit + 1);
+}
 
 void kv4_attention(const Kv4AttnArgs& a, int r0, int seqs, cudaStream_t stream) {
   if (seqs <= 0) return;
