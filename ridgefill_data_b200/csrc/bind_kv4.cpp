@@ -1,12 +1,12 @@
 // Python bindings of the 4-bit K/V cache (kv4.h). Everything a kernel indexes by is checked here for type,
 // device, layout and extent; positions and page ids, which live in device memory, are checked by the kernels.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
-#include <limits>
 #include <string>
 
 #include "kv4.h"
@@ -54,9 +54,8 @@ struct Cache {
     }
   }
 
-  int64_t rows(size_t r) const {
-    return std::min<int64_t>(pages[r].numel() * page_size, std::numeric_limits<int>::max());
-  }
+  // rows of a sequence: at most 2^30, so a split's first row fits an int
+  int64_t rows(size_t r) const { return std::min<int64_t>(pages[r].numel() * page_size, 1ll << 30); }
 
   // the last check before a launch, so that every other refusal holds on any device
   void on_gpu(const char* op) const { TORCH_CHECK(pool.is_cuda(), op, ": the cache must be on a CUDA device"); }
@@ -87,8 +86,9 @@ const int* first_rows(const OptT& row0, int64_t host, const Cache& c, int64_t T,
     return row0->data_ptr<int>();
   }
   TORCH_CHECK(c.pages.size() == 1, op, ": a host row0 serves one sequence");
-  TORCH_CHECK(host >= 0 && host + T <= c.rows(0), op, ": rows ", std::to_string(host), " .. ",
-              std::to_string(host + T), " of a cache that holds ", std::to_string(c.rows(0)));
+  TORCH_CHECK(host >= 0 && host <= c.rows(0) - T, op, ": rows ", std::to_string(host), " .. ",
+              std::to_string(static_cast<int64_t>(static_cast<uint64_t>(host) + T)), " of a cache that holds ",
+              std::to_string(c.rows(0)));
   return nullptr;
 }
 
@@ -100,8 +100,9 @@ OptT kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
   const int64_t R = (int64_t)c.pages.size();
   need(src, at::kBFloat16, c.pool, "src");
   const int64_t qw = hq * c.hd * (gated ? 2 : 1);
-  TORCH_CHECK(src.dim() == 2 && src.stride(1) == 1 && src.size(1) >= qw + 2 * c.hkv * c.hd && hq >= 0 && hq <= 65535,
-              "kv4.append: rows [*, q heads | k heads | v heads]");
+  TORCH_CHECK(src.dim() == 2 && src.stride(1) == 1 && hq >= 0 && hq + 2 * c.hkv <= 65535 &&
+                  src.size(1) >= qw + 2 * (int64_t)c.hkv * c.hd,
+              "kv4.append: rows [*, q heads | k heads | v heads], up to 65535 heads");
   TORCH_CHECK(aligned(src) && (src.size(0) <= 1 || src.stride(0) % 8 == 0) && small(src.stride(0)),
               "kv4.append: 16-byte aligned rows");
   TORCH_CHECK(R > 0 && src.size(0) % R == 0, "kv4.append: the same number of rows for every sequence");
@@ -141,7 +142,7 @@ OptT kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
     TORCH_CHECK(pos->dim() == 1 && pos->is_contiguous() && pos->numel() == src.size(0), "kv4.append: one position a row");
     a.pos = pos->data_ptr<int>();
   } else if (pos_offset >= 0) {
-    TORCH_CHECK(R == 1 && pos_offset + T < (1ll << 31), "kv4.append: pos_offset serves one sequence");
+    TORCH_CHECK(R == 1 && pos_offset < (1ll << 31) - T, "kv4.append: pos_offset serves one sequence");
   }
   if (rot > 0 && !pos.has_value() && !row0.has_value())
     TORCH_CHECK((pos_offset < 0 ? row0_host : pos_offset) + T <= a.table_rows,
@@ -151,8 +152,10 @@ OptT kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
     if (!q_out.has_value()) q_out = at::empty({src.size(0), hq, c.hd}, src.options());
     need(*q_out, at::kBFloat16, c.pool, "q_out");
     TORCH_CHECK(q_out->dim() == 3 && q_out->size(0) == src.size(0) && q_out->size(1) == hq && q_out->size(2) == c.hd &&
-                    q_out->stride(2) == 1 && small(q_out->stride(0)) && small(q_out->stride(1)) && q_out->stride(0) % 8 == 0 && q_out->stride(1) % 8 == 0 && aligned(*q_out),
+                    q_out->stride(2) == 1 && small(q_out->stride(0)) && small(q_out->stride(1)) &&
+                    q_out->stride(0) % 8 == 0 && q_out->stride(1) % 8 == 0 && aligned(*q_out),
                 "kv4.append: q_out [rows, q heads, head_dim], 16-byte aligned");
+    at::assert_no_internal_overlap(*q_out);
     a.q_out = bf(*q_out);
     a.q_out_row = (int)q_out->stride(0);
     a.q_out_head = (int)q_out->stride(1);
@@ -200,6 +203,7 @@ std::tuple<Tensor, Tensor> kv4_read(Tensor pool, std::vector<Tensor> pages, OptT
     TORCH_CHECK(t->numel() == 0 || (t->stride(3 - lead) == 1 && t->stride(2 - lead) == c.hd && t->stride(1 - lead) % 8 == 0 &&
                                     (single || t->stride(0) % 8 == 0) && t->strides() == k.strides() && aligned(*t)),
                 "kv4.read: k and v rows head_dim apart, 16-byte aligned, the same strides");
+    at::assert_no_internal_overlap(*t);
   }
   rf::Kv4ReadArgs a{};
   if (R == 0) return {k, v};
@@ -241,6 +245,7 @@ Tensor kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor po
   TORCH_CHECK(out.dim() == 2 && out.size(0) == R && out.size(1) == hq * c.hd && out.stride(1) == 1 && aligned(out) &&
                   (R <= 1 || out.stride(0) % 8 == 0),
               "kv4.attention: out [sequences, q heads * head_dim], 16-byte aligned");
+  at::assert_no_internal_overlap(out);
   rf::Kv4AttnArgs a{};
   if (gate.has_value()) {
     need(*gate, at::kBFloat16, c.pool, "gate");
@@ -269,7 +274,6 @@ Tensor kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor po
   a.out = bf(out);
   a.out_row = out.stride(0);
   a.splits = (int)S;
-  a.most = rf::kv4_most_splits(c.hd, c.hkv);
   a.most = rf::kv4_most_splits(c.hd, c.hkv);
   a.part_o = S > 1 ? parts.data_ptr<float>() : nullptr;
   a.part_ml = S > 1 ? a.part_o + R * S * hq * c.hd : nullptr;

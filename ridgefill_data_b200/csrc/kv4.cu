@@ -514,9 +514,9 @@ __device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs&
   const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
   if (first < 0) return;
   const int block0 = first / 16 + x;           // the block of the sequence
-  // its rows: row r is row t0 + r of the call
-  const int t0 = block0 * 16 - first;          // above -16; past 2^31 only where no row is left
-  if (t0 >= a.T || (long)block0 * 16 >= (1l << 31)) return;
+  const long behind = (long)block0 * 16 - first;
+  if (behind >= a.T || (long)block0 * 16 >= (1l << 31)) return;
+  const int t0 = (int)behind;                  // above -16: row r of the block is row t0 + r of the call
   const __nv_bfloat16* src = a.src + a.k_col + ((there ? head : 0) + (IS_V ? a.c.hkv : 0)) * HD + 16 * (lane % LANES);
   uint32_t v[2][8], w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   Place f[2];
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kReadWarps * 32) kv4_read_kernel(const __grid_
   const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
   // rows [lo, hi) of the block, in rows of the output behind t0
   const int block0 = first < 0 ? 0 : first / 16;
-  const int t0 = (block0 + x) * 16 - (first < 0 ? 0 : first);   // output row of the block's row 0
+  const int t0 = (int)((long)(block0 + x) * 16 - (first < 0 ? 0 : first));   // output row of the block's row 0
   const int lo = max(0, -t0), hi = min(16, a.n - t0);
   if (lo >= hi) return;
   const long row = (long)(block0 + x) * 16;
@@ -666,8 +666,6 @@ __global__ void __launch_bounds__(kReadWarps * 32) kv4_read_kernel(const __grid_
   }
 }
 
-}  // namespace
-
 template <int HD, int MODE, bool TURN>
 void launch_rows(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) {
   constexpr int HEADS = 512 / HD;
@@ -709,6 +707,8 @@ void launch_append(Kv4AppendArgs a, int r0, int seqs, cudaStream_t stream) {
     kv4_append_kernel<HD><<<dim3((rows + 7) / 8, heads), 256, 0, stream>>>(a, r0, rows, 0);
   count_launch();
 }
+
+}  // namespace
 
 void kv4_append(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) {
   if (seqs <= 0 || a.T <= 0) return;

@@ -51,7 +51,7 @@ __host__ __device__ constexpr int kv4_slot(int r) { return 4 * ((r & 7) >> 1) + 
 
 // The next kernel of the stream, if launched for it, may start before this one ends / wait until the previous one has ended
 // and its stores are seen (nothing to wait for where the launch did not allow an early start). A kernel that starts early
-// reads nothing before its wait that the previous one writes, and stores nothing.
+// touches no global memory before its wait: what the previous kernel wrote is seen after it only.
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -4,7 +4,13 @@
 //                     rows 0 .. pos, L depending on pos alone (the same bits alone or batched). A warp streams every
 //                     4th block of 16 keys through its own ring of bulk copies; no warp waits for another before the
 //                     end, where their states are joined in warp order into the split's partial (max, sum, output).
-// kv4_combine_kernel  grid (query head, sequence): the splits' partials in split order, the sum's division, the gate.
+// kv4_combine_kernel  grid (query head, sequence): the splits' partials in a fixed order, the sum's division, the gate. Both
+//                     start while the kernel before them ends.
+//
+// Bound by the cache's bytes: inside a CTA's loop DRAM runs at its rate, and what is above the floor is the CTAs' start (2 us:
+// position, page ids, query) and join (1.6 us), which the CTAs that share an SM reach together. B200: four streams behind
+// 128K rows of 8 heads of 128 130 us (680 MB: 104 at the measured 6.55 TB/s), eight behind up to 32K rows of 4 heads of 256
+// 46 us (190 MB: 29), one behind 16K rows of those 13 us (21 MB: 3.2; latency: 8 blocks a warp, one after another).
 //
 // Both products run on the tensor cores with the cache as the A operand (16 rows) and the G <= 8 query heads as its 8
 // columns, so nothing of a tile is wasted on absent query rows, and with the codes as they are stored: a masked nibble
@@ -31,7 +37,9 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 4;
 constexpr float kLow = -1e30f;   // below every score: exp2 of a difference to it is 0, never NaN
 
-constexpr int kUnit = 512;         // keys of a split, at least
+// Keys of a split, at least: a CTA's start and join take 4 us beside 1 us a block of each warp, so short splits cost batches
+// (256: eight behind up to 32K rows 52 us against 46) and long ones a single stream (1024: 23 us against 16 behind 16K).
+constexpr int kUnit = 512;
 constexpr int kTile = 128;         // and a multiple of this: every warp whole runs of blocks
 
 // keys of a split of rows 0 .. p when there may be `splits` of them
@@ -46,8 +54,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -55,8 +62,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 // the same with a zero accumulator
 __device__ __forceinline__ void mma_f16_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                             uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
@@ -193,6 +199,7 @@ struct QueryLoad {
   }
 };
 
+// The state of a warp over its keys. Fragment layouts as in mma.cuh: lane (g, t) = (lane / 4, lane % 4).
 template <int HD>
 struct Warp {
   using L = Kv4L<HD>;
@@ -392,6 +399,9 @@ struct Warp {
   }
 };
 
+// Two blocks a step where the registers allow (hd 64, 128: 147 -> 130 us for four streams behind 128K rows; a second chain
+// of dependent instructions beside the first); at hd 256 one, with the query's fragments left in shared memory for 3 CTAs
+// an SM. The ring holds what 12 to 24 warps an SM keep in flight: 124 to 185 KB.
 template <int HD>
 struct Cfg {
   static constexpr int NB = HD == 256 ? 1 : 2;          // blocks of a stage
@@ -414,13 +424,13 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
   const int s = blockIdx.x, g = blockIdx.y, sq = blockIdx.z, r = r0 + sq;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.hq / a.c.hkv;
+  if (lane < ST) mbar_init(bars[warp] + lane, NB);
+  fence_barrier_init();
   allow_next();
-  // before the previous kernel (this step's append, usually) has ended: positions and page ids alone, which it does not
-  // write; everything it may have written, and every store, after the wait
+  wait_previous();      // the previous kernel may have written any of this: rows, queries, positions, tables
   const int p = a.pos[r];
   if (p < 0 || p >= a.c.rows[sq]) {
     if (s > 0) return;
-    wait_previous();
     if (p >= 0 && g == 0 && threadIdx.x == 0) record_error(a.err, kErrBadIndex);
     for (int x = threadIdx.x; x < G * HD / 4; x += kWarps * 32)
       kv4_store<4>(a.out + (long)r * a.out_row + g * G * HD + 4 * x, {0.f, 0.f, 0.f, 0.f});
@@ -430,7 +440,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
   if (start > p) return;
   const int end = min(start + keys, p + 1);
   // the split's blocks in runs of NB: runs warp, warp + 4, ... Lane x of the first ST NB drives slot x of the ring: its
-  // copies, half of its stage's barrier, and the page id of the copy after next
+  // copies, its share of the stage's barrier, and the page id of the copy after next
   const int blocks = (end - start + 15) / 16;
   uint8_t* ring = smem + warp * ST * NB * L::BYTES;
   uint64_t* bar = bars[warp];
@@ -460,11 +470,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
     if (in >= per) in -= per, ++page;
     if (mine < blocks) id = __ldg(table + page);
   };
-  if (lane < ST) mbar_init(bar + lane, NB);
-  fence_barrier_init();
   __syncwarp();
   if (lane < ST * NB && mine < blocks) id = __ldg(table + page);
-  wait_previous();
   QueryLoad<HD> loading;
   loading.load(a, a.q + (long)r * a.q_row + (long)g * G * a.q_head, G, warp, lane);
   if (lane < ST * NB && mine - lane % NB < blocks) issue();

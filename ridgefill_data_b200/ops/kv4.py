@@ -14,7 +14,11 @@ or a row past the table records error code 7 (ops/_ext.py check_errors): append 
 zeros, attention leaves the page's rows out (a position past the table: a zero row).
 
 Rows are independent: appending a row again overwrites it, rows not appended keep their bytes. Two sequences may share
-pages that both only read; rows of one page appended by two calls at once must differ. Head dims 64, 128 and 256.
+pages that both only read; rows that one call, or two calls at once, append must be different rows of the pool. A
+sequence holds up to 2^30 rows. Head dims 64, 128 and 256.
+
+A call works on the current stream and allocates what it needs for itself, so calls on several streams and captured graphs
+share nothing but the pool.
 """
 from __future__ import annotations
 

@@ -170,6 +170,30 @@ def test_read_refuses():
         kv4.read(pool, table, 3, 0)
 
 
+def test_refuses_numbers_at_their_ends_and_outputs_on_themselves():
+    """Host numbers whose sum passes 64 bits, more heads than a launch has rows of blocks, outputs whose rows lie on each
+    other."""
+    pool, src, table = _args()
+    last = 2 ** 63 - 1
+    with pytest.raises(RuntimeError, match="rows 9223372036854775807"):
+        kv4.append(src, pool, [table], last, q_heads=4)
+    with pytest.raises(RuntimeError, match="rows 9223372036854775807"):
+        kv4.read(pool, table, 3, last)
+    with pytest.raises(RuntimeError, match="pos_offset"):
+        kv4.append(src, pool, [table], 0, q_heads=4, pos_offset=last)
+    with pytest.raises(RuntimeError, match="65535"):
+        kv4.append(torch.empty(1, 65535 * 64).bfloat16(), torch.zeros(1, 2, 1, 20 * 64 + 32, dtype=torch.uint8),
+                   [table], 0, q_heads=65532)
+    one = torch.zeros(1, 4, 128).bfloat16()
+    with pytest.raises(RuntimeError, match="memory location"):
+        kv4.append(src, pool, [table], 0, q_heads=4, q_out=one.expand(3, 4, 128))
+    with pytest.raises(RuntimeError, match="memory location"):
+        kv4.read(pool, table, 3, 0, out=(torch.zeros(1, 3, 128).bfloat16().expand(2, 3, 128),) * 2)
+    with pytest.raises(RuntimeError, match="memory location"):
+        kv4.attention(one.expand(2, 4, 128), pool, [table, table], torch.zeros(2, dtype=torch.int32), 0.1,
+                      out=torch.zeros(1, 512).bfloat16().expand(2, 512))
+
+
 def test_attention_refuses():
     pool, _, table = _args()
     q, pos = torch.zeros(1, 4, 128).bfloat16(), torch.zeros(1, dtype=torch.int32)

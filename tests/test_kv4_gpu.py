@@ -162,6 +162,59 @@ def test_append_skips_and_refuses_rows_on_the_device():
     assert same[:4].all() and same[12:].all() and not same[4:12].any()
 
 
+def test_append_of_many_rows_skips_and_refuses_on_the_device():
+    """The kernel for many rows: a skipped sequence, one past its table, a page id outside the pool, one in order; pages of
+    three blocks."""
+    hd, hkv, page, T = 128, 3, 48, 70
+    pages, total = _pages([96, 96, 96, 96], page)
+    pool = _random_pool(total, hkv, page, hd)
+    src = torch.randn(4 * T, 3 * hkv * hd, generator=torch.Generator().manual_seed(0)).bfloat16()
+    before = pool.cpu()
+    pages[2][1] = total
+    row0 = torch.tensor([-1, 50, 1, 7], dtype=torch.int32, device=DEV)
+    q = kv4.append(src.to(DEV), pool, pages, row0, q_heads=hkv)
+    assert _error() == 7
+    want = before.clone()
+    for s, r0 in enumerate((-1, 50, 1, 7)):
+        for t in range(T):
+            row = r0 + t
+            if r0 < 0 or row >= 96 or (s == 2 and row >= 48):
+                continue
+            n = s * T + t
+            for h in range(hkv):
+                ops.kv4_put(want[int(pages[s][row // page]), h, row % page // 16], row % 16,
+                            src[n, (hkv + h) * hd:(hkv + h + 1) * hd], src[n, (2 * hkv + h) * hd:(2 * hkv + h + 1) * hd])
+    assert torch.equal(pool.cpu(), want)
+    rows = src[:, :hkv * hd].to(DEV).view(4, T, hkv, hd)
+    got = q.view(4, T, hkv, hd)
+    assert got[0].eq(0).all() and got[1, 46:].eq(0).all() and torch.equal(got[1, :46], rows[1, :46])
+    assert torch.equal(got[3], rows[3])
+
+
+def test_append_of_many_rows_replayed_from_a_graph():
+    """Captured once, replayed with other rows at another first row and on other pages."""
+    hd, hkv, T = 64, 2, 100
+    pages, total = _pages([300, 300], 64)
+    pool, table = kv4.pool(total, hkv, 64, hd), pages[0].clone()
+    src = torch.randn(2, T, 3 * hkv * hd, device=DEV).bfloat16()
+    rows, row0 = src[0].clone(), torch.tensor([0], dtype=torch.int32, device=DEV)
+    kv4.append(rows, pool, [table], row0, q_heads=hkv)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q = kv4.append(rows, pool, [table], row0, q_heads=hkv)
+    for i, r0 in ((1, 150), (0, 33)):
+        pool.zero_()
+        rows.copy_(src[i])
+        row0.fill_(r0)
+        table.copy_(pages[i])
+        graph.replay()
+        want = kv4.pool(total, hkv, 64, hd)
+        want_q = kv4.append(src[i], want, pages[i], r0, q_heads=hkv)
+        assert torch.equal(pool, want) and torch.equal(q, want_q)
+    del graph
+
+
 def test_append_positions_apart_from_rows():
     """Rotary positions from a vector, an offset, or the cache row."""
     hd, T = 64, 9
@@ -420,12 +473,14 @@ def test_the_same_bits_alone_batched_and_on_other_pages():
     assert torch.equal(k, k[:1].expand_as(k))
 
 
-def test_decode_loop_replayed_from_a_graph_on_another_stream():
-    """append + attention captured once; the replays at new positions equal the eager calls bit for bit."""
-    hd, hkv, G, R, steps = 128, 2, 4, 3, 20
-    lens = [120, 5, 254]
+@pytest.mark.parametrize("lens", [[120, 5, 254], [1500, 5, 500]], ids=str)
+@pytest.mark.parametrize("hd", [128, 256])
+def test_decode_loop_replayed_from_a_graph_on_another_stream(hd, lens):
+    """append + attention (of one split and of several) captured once; the replays at new positions equal the eager calls
+    bit for bit."""
+    hkv, G, R, steps = 2, 4, 3, 20
     hq = hkv * G
-    tables = _tables(400, 64)
+    tables = _tables(1600, 64)
     g = torch.Generator(device=DEV).manual_seed(4)
     rows = [torch.randn(R, (2 * hq + 2 * hkv) * hd, device=DEV, generator=g).bfloat16() for _ in range(steps)]
     w = torch.randn(2, hd, device=DEV, generator=g).bfloat16()
@@ -462,6 +517,92 @@ def test_decode_loop_replayed_from_a_graph_on_another_stream():
     for s, n in enumerate(lens):
         for a, b in zip(kv4.read(pools[0], pages[s], n + steps), kv4.read(pools[1], pages[s], n + steps)):
             assert torch.equal(a, b)
+
+
+def test_steps_enqueued_without_a_pause():
+    """Append, attention and its join start before their predecessors end; a chain of dependent steps (each row made of the
+    last step's output, positions advanced on the device) enqueued at once equals the same steps with a pause after each."""
+    hd, hkv, R = 128, 2, 3
+    lens = [700, 40, 1300]
+    g = torch.Generator(device=DEV).manual_seed(8)
+    pages, total = _pages([n + 40 for n in lens], 128)
+    base = kv4.pool(total, hkv, 128, hd)
+    for s, n in enumerate(lens):
+        kv4.append(torch.randn(n, 2 * hkv * hd, device=DEV, generator=g).bfloat16(), base, [pages[s]], 0)
+    first = torch.randn(R, 4 * hd, device=DEV, generator=g).bfloat16()
+
+    def chain(pause):
+        pool, x, outs = base.clone(), first, []
+        pos = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        for _ in range(40):
+            q = kv4.append(torch.cat((x, x, x), 1)[:, :8 * hd], pool, pages, pos, q_heads=4)
+            x = kv4.attention(q, pool, pages, pos, 0.1)
+            outs.append(x)
+            x = (x + first).contiguous()
+            pos = pos + 1
+            if pause:
+                torch.cuda.synchronize()
+        return torch.stack(outs)
+    a, b = chain(False), chain(True)
+    assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_inputs_written_just_before():
+    """attention starts while the kernel before it ends: queries, positions and page tables that this kernel writes."""
+    pool, pages = _filled([700, 700], 2, 128, 128)
+    q = torch.randn(2, 8, 128, device=DEV).bfloat16()
+    table, other = pages
+    at = [torch.tensor([n], dtype=torch.int32, device=DEV) for n in (20, 699)]
+    want = {(i, j): kv4.attention(q[i:i + 1], pool, [pages[i]], at[j], 0.1) for i in range(2) for j in range(2)}
+    pos, now, mine = at[0].clone(), q[:1].clone(), table.clone()
+    for step in range(60):
+        i, j = step % 2, step // 2 % 2
+        now.copy_(q[i:i + 1]), mine.copy_(pages[i]), pos.copy_(at[j])
+        last = (lambda: pos.mul_(1), lambda: mine.mul_(1), lambda: now.mul_(1))[step % 3]
+        last()
+        assert torch.equal(kv4.attention(now, pool, [mine], pos, 0.1), want[i, j])
+    pos.fill_(0)
+    got = []
+    for n in range(0, 640, 20):
+        got.append(kv4.attention(now, pool, [mine], pos, 0.1))
+        pos.add_(20)
+    for n, o in zip(range(0, 640, 20), got):
+        assert torch.equal(o, kv4.attention(now, pool, [mine], torch.tensor([n], dtype=torch.int32, device=DEV), 0.1))
+
+
+def test_more_sequences_than_one_launch_takes():
+    """150 sequences of one page each: appended, attended and read in several launches, as each alone."""
+    hd, hkv, R = 64, 2, 150
+    pages = list(torch.randperm(R, generator=torch.Generator().manual_seed(1)).to(DEV, torch.int32).split(1))
+    pool = kv4.pool(R, hkv, 16, hd)
+    src = torch.randn(3 * R, 3 * hkv * hd, device=DEV).bfloat16()
+    row0 = (torch.arange(R, device=DEV) % 13).int()
+    q = kv4.append(src, pool, pages, row0, q_heads=hkv)
+    out = kv4.attention(q[2::3], pool, pages, row0 + 2, 0.2)
+    k, _ = kv4.read(pool, pages, 3, row0)
+    alone = kv4.pool(R, hkv, 16, hd)
+    for s in range(R):
+        one = kv4.append(src[3 * s:3 * s + 3], alone, pages[s], s % 13, q_heads=hkv)
+        assert torch.equal(q[3 * s:3 * s + 3], one)
+        assert torch.equal(out[s:s + 1], kv4.attention(one[2:], alone, [pages[s]], row0[s:s + 1] + 2, 0.2))
+        assert torch.equal(k[s], kv4.read(alone, pages[s], 3, s % 13)[0])
+    assert torch.equal(pool, alone)
+
+
+def test_two_streams_at_once():
+    """The same sequences attended from two streams at once: workspaces are each call's own."""
+    pool, pages = _filled([3000, 2000], 2, 128, 128)
+    pos = torch.tensor([2999, 1999], dtype=torch.int32, device=DEV)
+    qs = [torch.randn(2, 8, 128, device=DEV).bfloat16() for _ in range(2)]
+    want = [kv4.attention(q, pool, pages, pos, 0.1) for q in qs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(kv4.attention(qs[i], pool, pages, pos, 0.1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
 
 
 def test_pool_past_4_gib():
