@@ -14,6 +14,7 @@
 
 #include "kernels.h"
 
+#include <algorithm>
 #include <stdexcept>
 
 namespace rf {
@@ -21,6 +22,32 @@ namespace rf {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
+
+// Two 32-bit numbers under one instruction, each rounded as alone: half the issue slots, which bound the append.
+struct Two {
+  uint64_t w;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(w) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+  __device__ __forceinline__ explicit Two(uint32_t bf16_pair) : Two(bf16_lo(bf16_pair), bf16_hi(bf16_pair)) {}
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(w)); }
+};
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(c.w) : "l"(a.w), "l"(b.w), "l"(c.w));
+  return c;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(a.w) : "l"(a.w), "l"(b.w));
+  return a;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(a.w) : "l"(a.w), "l"(b.w));
+  return a;
+}
+__device__ __forceinline__ Two neg2(Two a) {
+  a.w ^= 0x8000000080000000ull;
+  return a;
+}
 
 // 1 / sqrt(m) to about 50 bits: two Newton steps on the 22 bits of the single-precision root.
 __device__ __forceinline__ double inverse_root(double m) {
@@ -33,6 +60,11 @@ __device__ __forceinline__ double inverse_root(double m) {
 
 __device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmul2_rn(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t fma_bf16(uint32_t a, uint32_t b, uint32_t c) {
+  const __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b),
+                                   *reinterpret_cast<__nv_bfloat162*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t add_bf16(uint32_t a, uint32_t b) {
@@ -59,40 +91,37 @@ struct Root {
     const double inv = inverse_root(m);
     rh = (float)inv, rl = (float)(inv - (double)rh);
   }
-  __device__ __forceinline__ float times(float v, float w, int mode) const {
-    float ph = rh, pl = rl;
-    if (mode == 1) {   // (1 + w) r as ph + pl
-      const float wh = 1.f + w, wl = w - (wh - 1.f);
-      ph = rh * wh, pl = fmaf(rl, wh, fmaf(rh, wl, fmaf(rh, wh, -ph)));
-    }
-    const float p = v * ph;
-    return p + fmaf(v, pl, fmaf(v, ph, -p));
-  }
   __device__ __forceinline__ uint32_t pair(uint32_t v, uint32_t w, int mode) const {
-    const uint32_t y = pack_bf16x2(times(bf16_lo(v), bf16_lo(w), mode), times(bf16_hi(v), bf16_hi(w), mode));
-    return mode == 0 ? mul_bf16(y, w) : y;
+    Two ph(rh), pl(rl);
+    if (mode == 1) {   // (1 + w) r as ph + pl
+      const Two h = ph, x(w), wh = add2(x, Two(1.f)), wl = fma2(add2(wh, Two(-1.f)), Two(-1.f), x);
+      ph = mul2(h, wh), pl = fma2(pl, wh, fma2(h, wl, fma2(h, wh, neg2(ph))));
+    }
+    const Two y(v), p = mul2(y, ph);
+    float a, b;
+    add2(p, fma2(y, pl, fma2(y, ph, neg2(p)))).get(a, b);
+    const uint32_t z = pack_bf16x2(a, b);
+    return mode == 0 ? mul_bf16(z, w) : z;
   }
 };
 
 // The same of a query, which is not quantised, in 32 bits: the arithmetic of head_norm_rope (norm.cu), bit for bit.
 __device__ __forceinline__ uint32_t query_pair(float inv, uint32_t v, uint32_t w, int mode) {
-  const float l = bf16_lo(v) * inv, h = bf16_hi(v) * inv;
-  return mode == 0 ? mul_bf16(pack_bf16x2(l, h), w)
-                   : pack_bf16x2(l * (1.f + bf16_lo(w)), h * (1.f + bf16_hi(w)));
+  Two y = mul2(Two(v), Two(inv));
+  if (mode == 1) y = mul2(y, add2(Two(w), Two(1.f)));
+  float a, b;
+  y.get(a, b);
+  const uint32_t z = pack_bf16x2(a, b);
+  return mode == 0 ? mul_bf16(z, w) : z;
 }
 
+// NaN where either is
 __device__ __forceinline__ uint32_t min_bf16(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  const __nv_bfloat162 r = __hmin2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// larger magnitude, NaN where either is
-__device__ __forceinline__ uint32_t top_bf16(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
-  return r;
-}
 __device__ __forceinline__ uint32_t max_bf16(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
@@ -116,16 +145,20 @@ struct Steps {
   __device__ __forceinline__ void codes(const uint32_t* pairs, uint32_t* words) const {
     constexpr float kBase = 12582912.f;            // its bits: 0x4b400000
     const float inv = sf == 0.f ? 0.f : __fdividef(1.f, sf);
-    float c[N];
+    Two c[N / 2];
+    const Two size2(size), m2(-mf), s2(-sf), inv2(inv);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float d = fmaf(j & 1 ? bf16_hi(pairs[j / 2]) : bf16_lo(pairs[j / 2]), size, -mf);
-      const float q = d * inv;
-      c[j] = fmaf(fmaf(-q, sf, d), inv, q);
+    for (int j = 0; j < N / 2; ++j) {
+      const Two d = fma2(Two(pairs[j]), size2, m2), q = mul2(d, inv2);
+      c[j] = fma2(fma2(q, s2, d), inv2, q);
     }
     if (sf < 0x1p-13f) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) c[j] = fminf(fmaxf(c[j], 0.f), 15.f);
+      for (int j = 0; j < N / 2; ++j) {
+        float x, y;
+        c[j].get(x, y);
+        c[j] = Two(fminf(fmaxf(x, 0.f), 15.f), fminf(fmaxf(y, 0.f), 15.f));
+      }
     }
     uint32_t base = 0;                             // the sum of the bases by 16^j
 #pragma unroll
@@ -133,7 +166,12 @@ struct Steps {
 #pragma unroll
     for (int x = 0; x < (N + 7) / 8; ++x) words[x] = 0u - base;
 #pragma unroll
-    for (int j = 0; j < N; ++j) words[j / 8] += __float_as_uint(c[j] + kBase) << (4 * (j & 7));
+    for (int j = 0; j < N / 2; ++j) {
+      float x, y;
+      add2(c[j], Two(kBase)).get(x, y);
+      words[j / 4] += __float_as_uint(x) << (8 * (j & 3));
+      words[j / 4] += __float_as_uint(y) << (8 * (j & 3) + 4);
+    }
   }
 };
 
@@ -336,13 +374,20 @@ __global__ void __launch_bounds__(256)
 // Many rows: the queries and the cached rows go their own ways in one launch (kv4_append_rows_kernel).
 //
 // query_rows            a lane holds 8 values (16 bytes), so a warp's loads and stores are whole sectors whatever the head
-//                       size: 256 / hd heads of a row at a time, two times. The rotation's half is whole lanes (rot / 2 a
-//                       multiple of 8).
+//                       size: 256 / hd heads of a row at a time. The rotation's half is whole lanes (rot / 2 a multiple of
+//                       8).
 // cache_block           a CTA per block of 16 cache rows and 512 / hd heads of K or of V, a warp two rows: a lane holds 16
 //                       values (half a group), hd / 16 lanes a head, so what is done once a head or a group is done for all
-//                       its heads at once; the block's bytes are put together in shared memory and leave as 16-byte pieces (row by row
-//                       they would be 24 partial sectors a row and head). A block that is only partly appended is written
-//                       in place, row by row. The rotation's half is whole lanes (rot / 2 a multiple of 16).
+//                       its heads at once; the block's bytes are put together in shared memory and leave as 16-byte pieces
+//                       (row by row they would be 24 partial sectors a row and head). A block that is only partly appended
+//                       is written in place, row by row. The rotation's half is whole lanes (rot / 2 a multiple of 16).
+//
+// Both load the rows, the page's id and the rotation's entries before anything waits for one of them (80 -> 72 us for the
+// queries; behind one another each costs a trip to memory with 32 warps an SM to cover it). Bound by the instructions of the
+// cached rows (16 values of a lane: 190, 86 of them the codes) next to the queries' bytes. B200, 16384 rows: 32 q and 8 KV
+// heads of 128 74 us (356 MB: 54 at the measured 6.55 TB/s), the KV heads alone 37 (88 MB: 13.5); 24 gated and 4 of 256
+// with norms 109 us (491 MB: 75). Tried: row pieces through a ring of asynchronous copies (equal), the next wave's rows
+// fetched to L2 ahead (84 us), 3 CTAs an SM of 80 registers (82 us).
 
 // kept out of line: the common cases branch past it
 __device__ __noinline__ int divide(int a, int b) { return a / b; }
@@ -360,48 +405,61 @@ __device__ __forceinline__ Place place(const Kv4AppendArgs& a, int first, int sq
   return f;
 }
 
-// 16 rows of 2 x 256 / hd query heads: a warp two rows, their loads in flight together.
+// A piece of the query rows: a warp takes US rows of YS x 256 / hd heads, their loads in flight together. What is done once
+// a row serves as many heads as fit the registers; at hd 64 fewer, since models of such heads have few.
+template <int HD>
+struct QPiece {
+  static constexpr int LANES = HD / 8, HEADS = 32 / LANES, YS = HD == 64 ? 2 : 4, US = 4 / YS;
+  static constexpr int ROWS = 8 * US, SET = YS * HEADS;
+};
+
 template <int HD, int MODE, bool TURN>
 __device__ __forceinline__ void query_rows(const Kv4AppendArgs& a, int r0, int rows, int x, int set) {
-  constexpr int LANES = HD / 8, HEADS = 32 / LANES;
+  using Q = QPiece<HD>;
+  constexpr int LANES = Q::LANES, HEADS = Q::HEADS, YS = Q::YS, US = Q::US;
   const int lane = threadIdx.x & 31, j = lane % LANES;
-  const int n0 = x * 16 + (threadIdx.x >> 5);
+  const int n0 = x * Q::ROWS + (threadIdx.x >> 5);
   if (n0 >= rows) return;
-  const int head = set * 2 * HEADS + lane / LANES;   // and HEADS further
-  const bool there[2] = {head < a.hq, head + HEADS < a.hq};
-  Row<8> v[2][2], w;
+  const int head = set * Q::SET + lane / LANES;   // and HEADS, 2 HEADS, .. further
+  Row<8> v[US][YS], w;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < US; ++u) {
     const int src_row = r0 * a.T + min(n0 + 8 * u, rows - 1);
     const __nv_bfloat16* src = a.src + (long)src_row * a.src_row + 8 * j;
 #pragma unroll
-    for (int y = 0; y < 2; ++y) v[u][y].load(src + (there[y] ? (head + y * HEADS) * a.q_stride : 0));
+    for (int y = 0; y < YS; ++y) v[u][y].load(src + (head + y * HEADS < a.hq ? (head + y * HEADS) * a.q_stride : 0));
   }
   if constexpr (MODE >= 0) w.load(a.q_norm + 8 * j);
   const int h = a.rot / 2, i0 = 8 * j;
   const bool low = i0 < h;
-  Turn<8> turn;
-  turn.in = i0 < a.rot;
-  turn.from = !turn.in ? lane : low ? lane + h / 8 : lane - h / 8;
+  Turn<8> turn[US];
+  Place f[US];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < US; ++u) {
+    const int n = min(n0 + 8 * u, rows - 1);
+    int sq = 0, t = n;
+    if (t >= a.T) sq = divide(n, a.T), t = n - sq * a.T;
+    f[u] = place(a, a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host, sq, t, r0 * a.T + n);
+    turn[u].in = i0 < a.rot;
+    turn[u].from = !turn[u].in ? lane : low ? lane + h / 8 : lane - h / 8;
+    if constexpr (TURN) {
+      const long entry = f[u].ok && turn[u].in ? (long)f[u].p * h + (low ? i0 : i0 - h) : 0;
+      turn[u].c.load(a.cos + entry);
+      turn[u].s.load(a.sin + entry);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < US; ++u) {
     const int n = n0 + 8 * u;
     if (n >= rows) break;
     const int src_row = r0 * a.T + n;
-    int sq = 0, t = n;
-    if (t >= a.T) sq = divide(n, a.T), t = n - sq * a.T;
-    const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
-    const Place f = place(a, first, sq, t, src_row);
     if constexpr (TURN) {
-      const long entry = f.ok && turn.in ? (long)f.p * h + (low ? i0 : i0 - h) : 0;
-      turn.c.load(a.cos + entry);
-      turn.s.load(a.sin + entry);
 #pragma unroll
-      for (int z = 0; z < 4; ++z) turn.s.w[z] ^= low ? 0x80008000u : 0u;
+      for (int z = 0; z < 4; ++z) turn[u].s.w[z] ^= low ? 0x80008000u : 0u;
     }
-    __nv_bfloat16* dst = a.q_out + (long)src_row * a.q_out_row + 8 * j;
+    __nv_bfloat16* dst = a.q_out + (long)src_row * a.q_out_row + (long)head * a.q_out_head + 8 * j;
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
+    for (int y = 0; y < YS; ++y) {
       Row<8>& q = v[u][y];
       if constexpr (MODE >= 0) {
         // the sums of the hd / 32 values that a lane holds when a warp takes one head, added across in that order too:
@@ -424,67 +482,69 @@ __device__ __forceinline__ void query_rows(const Kv4AppendArgs& a, int r0, int r
 #pragma unroll
         for (int y = 0; y < 4; ++y) q.w[y] = query_pair(inv, q.w[y], w.w[y], MODE);
       }
-      if constexpr (TURN) turn.apply(q);
-      if (!f.ok) q.w[0] = q.w[1] = q.w[2] = q.w[3] = 0;
-      if (there[y]) q.store(dst + (long)(head + y * HEADS) * a.q_out_head);
+      if constexpr (TURN) turn[u].apply(q);
+      if (!f[u].ok) q.w[0] = q.w[1] = q.w[2] = q.w[3] = 0;
+      if (head + y * HEADS < a.hq) q.store(dst + (long)(y * HEADS) * a.q_out_head);
     }
   }
 }
 
-// One row of a warp's heads of K (or V), quantised to `block`, its head's block.
-template <int HD, bool IS_V, int MODE, bool TURN>
-__device__ __forceinline__ void cache_row(uint32_t (&v)[8], const Kv4AppendArgs& a, const uint32_t (&w)[8], const Place& f,
-                                          uint8_t* block, bool there, int r, int lane) {
-  using L = Kv4L<HD>;
-  constexpr int LANES = HD / 16;
-  const int j = lane % LANES;                  // lane of its head
-  if constexpr (MODE >= 0) {
-    double ss = 0.0;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const double l = low_double(v[x]), h = high_double(v[x]);
-      ss = fma(h, h, fma(l, l, ss));
-    }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-    const Root root(ss * (1.0 / HD) + a.eps);
-#pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = root.pair(v[x], w[x], MODE);
+// 16 values of a lane in place of Turn: entries of the tables at one position, loaded while the row before is quantised.
+struct Turn16 {
+  uint4 c[2], s[2];
+  int at, from;            // first entry, lane of the partners
+  bool inside;
+  uint32_t sign;           // -1 in the first half, as bf16 pairs
+
+  __device__ __forceinline__ Turn16(int rot, int lane, int j) {
+    const int half = rot / 32;                 // lanes of half the rotated values
+    const bool low = j < half;
+    inside = j < 2 * half;
+    at = !inside ? 0 : 16 * (low ? j : j - half);
+    from = !inside ? lane : low ? lane + half : lane - half;
+    sign = low ? 0xbf80bf80u : 0x3f803f80u;
   }
-  if constexpr (TURN) {
-    const int half = a.rot / 32;               // lanes of half the rotated values
-    const bool inside = j < 2 * half, low = j < half;
-    const int from = !inside ? lane : low ? lane + half : lane - half;
-    const uint32_t sign = low ? 0x80008000u : 0u;
-    const long e = inside ? (long)f.p * (a.rot / 2) + 16 * (low ? j : j - half) : 0;
+  __device__ __forceinline__ void load(const Kv4AppendArgs& a, int p) {
+    const long e = (long)p * (a.rot / 2) + at;
     const uint4* cp = reinterpret_cast<const uint4*>(a.cos + e);
     const uint4* sp = reinterpret_cast<const uint4*>(a.sin + e);
-    const uint4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
-    const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    const uint32_t s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+    c[0] = __ldg(cp), c[1] = __ldg(cp + 1), s[0] = __ldg(sp), s[1] = __ldg(sp + 1);
+  }
+  __device__ __forceinline__ void apply(uint32_t (&v)[8]) const {
+    const uint32_t cw[8] = {c[0].x, c[0].y, c[0].z, c[0].w, c[1].x, c[1].y, c[1].z, c[1].w};
+    const uint32_t sw[8] = {s[0].x, s[0].y, s[0].z, s[0].w, s[1].x, s[1].y, s[1].z, s[1].w};
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      const uint32_t other = __shfl_sync(kFull, v[x], from) ^ sign;
-      const uint32_t y = add_bf16(mul_bf16(v[x], c[x]), mul_bf16(other, s[x]));
+      const uint32_t other = __shfl_sync(kFull, v[x], from);
+      const uint32_t y = fma_bf16(mul_bf16(other, sw[x]), sign, mul_bf16(v[x], cw[x]));   // a product with +-1 is exact
       v[x] = inside ? y : v[x];
     }
   }
-  // the head's largest magnitude, then the group's ends over its two lanes
-  unsigned top = top_bf16(top_bf16(top_bf16(v[0], v[1]), top_bf16(v[2], v[3])),
-                          top_bf16(top_bf16(v[4], v[5]), top_bf16(v[6], v[7])));
-  top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
-  const bool bad = top >= 0x5b80u;             // 2^56 and above, infinities and NaN
-  if (bad)
-#pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = 0;
-  const int e = top == 0 ? 0 : max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
+};
+
+// One row of a warp's heads of K (or V), quantised to `block`, its head's block.
+template <int HD, bool IS_V>
+__device__ __forceinline__ void put_heads(uint32_t (&v)[8], uint8_t* block, bool there, int r, int lane) {
+  using L = Kv4L<HD>;
+  constexpr int LANES = HD / 16;
+  const int j = lane % LANES;                  // lane of its head
+  // the group's ends over its two lanes, and from them the head's largest magnitude; NaN is kept on the way
   uint32_t least = v[0], most = v[0];
 #pragma unroll
   for (int x = 1; x < 8; ++x) least = min_bf16(least, v[x]), most = max_bf16(most, v[x]);
   least = min_bf16(least, __shfl_xor_sync(kFull, least, 1));
   most = max_bf16(most, __shfl_xor_sync(kFull, most, 1));
+  unsigned top = __vmaxu2(least & 0x7fff7fffu, most & 0x7fff7fffu);
+  top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+  for (int o = LANES / 2; o > 1; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
+  const bool bad = top >= 0x5b80u;             // 2^56 and above, infinities and NaN
+  if (bad) {
+    least = most = 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = 0;
+  }
+  const int e = top == 0 ? 0 : max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
   const Steps st(fminf(bf16_lo(least), bf16_hi(least)), fmaxf(bf16_lo(most), bf16_hi(most)), kv4_pow2(-e));
   uint32_t codes[2];
   st.codes<16>(v, codes);
@@ -517,45 +577,73 @@ __device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs&
   const long behind = (long)block0 * 16 - first;
   if (behind >= a.T || (long)block0 * 16 >= (1l << 31)) return;
   const int t0 = (int)behind;                  // above -16: row r of the block is row t0 + r of the call
-  const __nv_bfloat16* src = a.src + a.k_col + ((there ? head : 0) + (IS_V ? a.c.hkv : 0)) * HD + 16 * (lane % LANES);
-  uint32_t v[2][8], w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  Place f[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int t = t0 + warp + 8 * u;
-    const bool mine = t >= 0 && t < a.T;
-    const int src_row = (r0 + sq) * a.T + (mine ? t : 0);
-    const uint4* at = reinterpret_cast<const uint4*>(src + (long)src_row * a.src_row);
-    const uint4 y = __ldg(at), z = __ldg(at + 1);
-    v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w, v[u][4] = z.x, v[u][5] = z.y, v[u][6] = z.z, v[u][7] = z.w;
-    f[u] = place(a, first, sq, t, src_row);
-    if (!mine) f[u].row = -1, f[u].ok = false;
-  }
-  if constexpr (MODE >= 0) {
-    const uint4* wp = reinterpret_cast<const uint4*>(a.k_norm + 16 * (lane % LANES));
-    const uint4 y = __ldg(wp), z = __ldg(wp + 1);
-    w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w, w[4] = z.x, w[5] = z.y, w[6] = z.z, w[7] = z.w;
-  }
+  const int src0 = (r0 + sq) * a.T;
   const int per = a.c.page_size / 16;
   const int nth = a.page_shift >= 0 ? block0 >> (a.page_shift - 4) : divide(block0, per);
   int id = -1;
   if (block0 * 16 < a.c.rows[sq]) id = __ldg(a.c.pages[sq] + nth);
-  const bool page = id >= 0 && id < a.c.num_pages;
-  const int pitch = per * L::BYTES;            // between KV heads (a page of a head is below 2^31 bytes)
-  uint8_t* out = a.c.pool + (long)((page ? id : 0) * (long)a.c.hkv + set * HEADS) * pitch + (block0 - nth * per) * L::BYTES;
-  // every row here and in order: through shared memory
-  const bool whole = __syncthreads_and(f[0].ok && f[1].ok && page);
+  const __nv_bfloat16* src = a.src + a.k_col + ((there ? head : 0) + (IS_V ? a.c.hkv : 0)) * HD + 16 * (lane % LANES);
+  uint32_t v[2][8];
+  const int p0 = a.pos_offset >= 0 ? a.pos_offset + t0 : block0 * 16;
+  int p[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    if (!whole && !(f[u].ok && page)) {
-      if (f[u].row >= 0 && lane == 0) record_error(a.err, kErrBadIndex);
-      continue;
+    const int r = warp + 8 * u, t = t0 + r, src_row = src0 + (t >= 0 && t < a.T ? t : 0);
+    const uint4* at = reinterpret_cast<const uint4*>(src + (long)src_row * a.src_row);
+    const uint4 y = __ldg(at), z = __ldg(at + 1);
+    v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w, v[u][4] = z.x, v[u][5] = z.y, v[u][6] = z.z, v[u][7] = z.w;
+    p[u] = a.pos != nullptr ? __ldg(a.pos + src_row) : p0 + r;
+  }
+  // every row of the block here, within the table and at a rotary position of the tables: through shared memory
+  bool whole = t0 >= 0 && t0 + 16 <= a.T && block0 * 16 < a.c.rows[sq];
+  if (whole && a.rot > 0)
+    whole = a.pos == nullptr ? p0 <= a.table_rows - 16
+                             : __all_sync(kFull, (unsigned)__ldg(a.pos + src0 + t0 + (lane & 15)) < (unsigned)a.table_rows);
+  Turn16 turn(a.rot, lane, lane % LANES);
+  if constexpr (TURN) turn.load(a, (unsigned)p[0] < (unsigned)a.table_rows ? p[0] : 0);
+  const int pitch = per * L::BYTES;            // between KV heads (a page of a head is below 2^31 bytes)
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if constexpr (MODE >= 0) {
+      double ss = 0.0, sh = 0.0;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const double l = low_double(v[u][x]), h = high_double(v[u][x]);
+        ss = fma(l, l, ss), sh = fma(h, h, sh);
+      }
+      ss += sh;
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+      const Root root(ss * (1.0 / HD) + a.eps);
+      const uint4* wp = reinterpret_cast<const uint4*>(a.k_norm + 16 * (lane % LANES));
+      const uint4 y = __ldg(wp), z = __ldg(wp + 1);
+      const uint32_t w[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[u][x] = root.pair(v[u][x], w[x], MODE);
     }
-    uint8_t* block = whole ? image + (lane / LANES) * L::BYTES : out + (long)(lane / LANES) * pitch;
-    cache_row<HD, IS_V, MODE, TURN>(v[u], a, w, f[u], block, there, warp + 8 * u, lane);
+    if constexpr (TURN) {
+      turn.apply(v[u]);
+      if (u == 0) turn.load(a, (unsigned)p[1] < (unsigned)a.table_rows ? p[1] : 0);
+    }
+    const int r = warp + 8 * u, t = t0 + r;
+    uint8_t* block = image + (lane / LANES) * L::BYTES;
+    if (!whole) {                              // row by row, each where it belongs
+      if (t < 0 || t >= a.T) continue;
+      if (id < 0 || id >= a.c.num_pages || (a.rot > 0 && (unsigned)p[u] >= (unsigned)a.table_rows)) {
+        if (lane == 0) record_error(a.err, kErrBadIndex);
+        continue;
+      }
+      block = a.c.pool + ((long)id * a.c.hkv + head) * pitch + (block0 - nth * per) * L::BYTES;
+    }
+    put_heads<HD, IS_V>(v[u], block, there, r, lane);
   }
   if (!whole) return;
   __syncthreads();
+  if (id < 0 || id >= a.c.num_pages) {
+    if (threadIdx.x == 0) record_error(a.err, kErrBadIndex);
+    return;
+  }
+  uint8_t* out = a.c.pool + ((long)id * a.c.hkv + set * HEADS) * pitch + (block0 - nth * per) * L::BYTES;
   // K: codes, s and m, exponents; V: the same, each behind K's
   constexpr int CODES = HD / 2, PARAMS = HD / 8, PIECES = CODES + PARAMS + 1;
   const int heads = min(HEADS, a.c.hkv - set * HEADS);
@@ -568,11 +656,21 @@ __device__ __forceinline__ void cache_block(uint8_t* image, const Kv4AppendArgs&
   }
 }
 
+// n / d for 32-bit n by a product: m = (2^64 + e) / d with e < d makes it n / d + n e / (d 2^64), less than 1 / d above. (The
+// compiler's divisions, one of them in 64 bits, were a twelfth of the kernel's instructions.)
+struct Divisor {
+  unsigned d;
+  unsigned long long m;
+  explicit Divisor(unsigned d_ = 1) : d(d_), m(d_ == 1 ? 0 : ~0ull / d_ + 1) {}
+  __device__ __forceinline__ unsigned of(unsigned n) const { return m == 0 ? n : (unsigned)__umul64hi(n, m); }
+};
+
 // Queries (bound by their bytes) and cached rows (bound by their arithmetic) of one call side by side: CTA i takes a block of
 // the cache when i kv / (q + kv) reaches its next whole number, else query rows.
 struct AppendPlan {
-  int q_rows, q_sets;          // CTAs of the queries: 16-row pieces, sets of heads
-  int spans, kv_sets, seqs;    // of the cache: blocks of a sequence, 2 x sets of KV heads, sequences
+  Divisor q_sets;              // of the queries: sets of heads
+  Divisor kv_sets, spans;      // of the cache: 2 x sets of KV heads, blocks of a sequence
+  unsigned long long share;    // 2^32 kv / (q + kv), rounded up: i share / 2^32 counts up to kv
 };
 
 template <int HD, int MODE, bool TURN>
@@ -580,18 +678,18 @@ __global__ void __launch_bounds__(256, 4)
     kv4_append_rows_kernel(const __grid_constant__ Kv4AppendArgs a, int r0, int rows, const AppendPlan plan) {
   __shared__ __align__(16) uint8_t image[512 / HD * Kv4L<HD>::BYTES];
   allow_next();
-  const unsigned kv = (unsigned)plan.spans * plan.kv_sets * plan.seqs, all = gridDim.x, i = blockIdx.x;
-  const unsigned at = (unsigned)((unsigned long long)i * kv / all);
-  if ((unsigned)((unsigned long long)(i + 1) * kv / all) > at) {
+  const unsigned i = blockIdx.x, at = (unsigned)(i * plan.share >> 32);
+  if ((unsigned)((i + 1) * plan.share >> 32) > at) {
     // kv sets of one block side by side: they share the rows of the source
-    const int set = at % plan.kv_sets, x = at / plan.kv_sets % plan.spans, sq = at / plan.kv_sets / plan.spans;
+    const unsigned span = plan.kv_sets.of(at), set = at - span * plan.kv_sets.d;
+    const unsigned sq = plan.spans.of(span), x = span - sq * plan.spans.d;
     if (set & 1)
       cache_block<HD, true, -1, false>(image, a, r0, sq, x, set / 2);
     else
       cache_block<HD, false, MODE, TURN>(image, a, r0, sq, x, set / 2);
   } else {
-    const int q = i - at;
-    query_rows<HD, MODE, TURN>(a, r0, rows, q / plan.q_sets, q % plan.q_sets);
+    const unsigned q = i - at, n = plan.q_sets.of(q);
+    query_rows<HD, MODE, TURN>(a, r0, rows, n, q - n * plan.q_sets.d);
   }
 }
 
@@ -670,14 +768,13 @@ template <int HD, int MODE, bool TURN>
 void launch_rows(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) {
   constexpr int HEADS = 512 / HD;
   const int rows = seqs * a.T;
-  AppendPlan plan{};
-  plan.q_rows = (rows + 15) / 16;
-  plan.q_sets = (a.hq + HEADS - 1) / HEADS;
+  using Q = QPiece<HD>;
+  const unsigned q_sets = (a.hq + Q::SET - 1) / Q::SET, kv_sets = 2 * ((a.c.hkv + HEADS - 1) / HEADS);
   // blocks that T rows can touch: known exactly for a host row, else one more
-  plan.spans = a.row0 == nullptr ? (int)(((long)a.row0_host + a.T - 1) / 16 - a.row0_host / 16 + 1) : (a.T + 14) / 16 + 1;
-  plan.kv_sets = 2 * ((a.c.hkv + HEADS - 1) / HEADS);
-  plan.seqs = seqs;
-  const unsigned grid = (unsigned)plan.q_rows * plan.q_sets + (unsigned)plan.spans * plan.kv_sets * seqs;
+  const unsigned spans = a.row0 == nullptr ? (unsigned)(((long)a.row0_host + a.T - 1) / 16 - a.row0_host / 16 + 1)
+                                           : (unsigned)(a.T + 14) / 16 + 1;
+  const unsigned kv = spans * kv_sets * seqs, grid = (unsigned)((rows + Q::ROWS - 1) / Q::ROWS) * q_sets + kv;
+  AppendPlan plan{Divisor(std::max(q_sets, 1u)), Divisor(kv_sets), Divisor(spans), (((unsigned long long)kv << 32) + grid - 1) / grid};
   kv4_append_rows_kernel<HD, MODE, TURN><<<grid, 256, 0, stream>>>(a, r0, rows, plan);
   count_launch();
 }
@@ -688,9 +785,10 @@ void launch_append(Kv4AppendArgs a, int r0, int seqs, cudaStream_t stream) {
   a.page_shift = -1;
   for (int j = 4; j < 31; ++j)
     if (a.c.page_size == 1 << j) a.page_shift = j;
-  // From 64 rows of a sequence on (four blocks of the cache) the kernels for many rows; fewer: a warp a row and head, one
-  // launch and the shorter way through a row.
-  if (a.T >= 64 && a.rot % 32 == 0) {
+  // From 256 rows on, in whole blocks' worth, the kernel for many rows; fewer: a warp a row and head, the shorter way through
+  // a row. (32 + 8 heads of 128, many / few: 128 rows 3.5 / 3.3 us, 256 rows 4.1 / 4.7, 1024 rows 6.5 / 12.7; 16 sequences
+  // of 8 rows 3.6 / 3.5, of 16 rows 3.9 / 5.0. 24 + 4 heads of 256 with norms: 256 rows 5.3 / 5.2, 1024 rows 10.0 / 12.7.)
+  if (a.T >= 16 && rows >= 256 && a.rot % 32 == 0) {
     switch ((a.norm_mode + 1) * 2 + (a.rot > 0)) {
       case 0: launch_rows<HD, -1, false>(a, r0, seqs, stream); break;
       case 1: launch_rows<HD, -1, true>(a, r0, seqs, stream); break;

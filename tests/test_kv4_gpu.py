@@ -63,6 +63,15 @@ APPEND = [
     (256, 3, 2, False, 0, 64, 128, [200], 80),
     (64, 5, 1, False, 1, 16, 32, [3], 100),
     (128, 2, 2, False, -1, 0, 128, [0], 64),
+    # 256 rows and more
+    (128, 3, 5, True, 1, 64, 48, [5, 90], 140),
+    (256, 3, 2, False, 0, 64, 128, [200], 300),
+    (64, 5, 1, False, 1, 32, 32, [3], 261),
+    (64, 2, 8, False, 0, 64, 80, [16, 0, 9], 99),
+    (128, 2, 2, False, -1, 0, 128, [0], 256),
+    (256, 1, 3, False, -1, 256, 32, [31], 266),
+    (256, 2, 6, True, 1, 64, 128, [130], 257),
+    (128, 1, 8, False, 0, 128, 64, list(range(0, 60, 3)), 16),
 ]
 
 
@@ -102,6 +111,34 @@ def test_append_writes_the_oracles_bytes_and_no_others(case):
         assert torch.equal(q, want_q)
     else:
         assert q is None
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_append_of_many_extreme_rows(hd):
+    """The same rows through the kernel for many rows: every block as the one that the kernel for few rows writes."""
+    y = torch.randn(16, hd, generator=torch.Generator().manual_seed(4)).bfloat16()
+    y[0], y[1], y[2] = 0.0, -0.0, -7.25
+    y[3], y[3, 9] = 0.0, -5.0
+    y[4, 0], y[5, hd - 1], y[6, 40] = math.inf, -math.inf, math.nan
+    y[7] *= 2.0 ** 54
+    y[8, 3] = -(2.0 ** 56)
+    y[9] *= 1e-38
+    y[10] *= 2.0 ** -41
+    y[11, 5] = 2.0 ** 55.9
+    y[12] = 1e-40
+    y[13, 32:64] = 3.0
+    y[14, 33], y[14, 34] = -math.nan, math.inf
+    heads = [y.roll(i, 0) for i in range(6)]                       # 3 KV heads of K, then of V
+    src = torch.cat(heads, 1).to(DEV)
+    few, many = _random_pool(1, 3, 16, hd), _random_pool(17, 3, 16, hd)
+    kv4.append(src, few, torch.zeros(1, dtype=torch.int32, device=DEV), 0)
+    want = torch.zeros(3, kv4.block_bytes(hd), dtype=torch.uint8)
+    for h in range(3):
+        for r in range(16):
+            ops.kv4_put(want[h], r, heads[h][r], heads[3 + h][r])
+    assert torch.equal(few.cpu()[0, :, 0], want)
+    kv4.append(src.repeat(17, 1), many, torch.arange(17, dtype=torch.int32, device=DEV), 0)
+    assert torch.equal(many, few.expand(17, -1, -1, -1))
 
 
 def test_append_extreme_rows():
@@ -191,10 +228,11 @@ def test_append_of_many_rows_skips_and_refuses_on_the_device():
     assert torch.equal(got[3], rows[3])
 
 
-def test_append_of_many_rows_replayed_from_a_graph():
+@pytest.mark.parametrize("T", [100, 300])
+def test_append_of_many_rows_replayed_from_a_graph(T):
     """Captured once, replayed with other rows at another first row and on other pages."""
-    hd, hkv, T = 64, 2, 100
-    pages, total = _pages([300, 300], 64)
+    hd, hkv = 64, 2
+    pages, total = _pages([500, 500], 64)
     pool, table = kv4.pool(total, hkv, 64, hd), pages[0].clone()
     src = torch.randn(2, T, 3 * hkv * hd, device=DEV).bfloat16()
     rows, row0 = src[0].clone(), torch.tensor([0], dtype=torch.int32, device=DEV)
