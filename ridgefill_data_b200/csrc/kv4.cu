@@ -3,8 +3,8 @@
 // kv4_append_kernel  a warp per row and head (q | k | v), a lane holding hd / 32 consecutive values: head norm and rotation
 //                    (q, k), then q goes out in bf16 and k / v rows are quantised into their block.
 // kv4_append_rows_kernel  the same for many rows (below).
-// kv4_read_kernel    one warp per block of 16 rows: the block to shared memory in 16-byte pieces, then row by row the values
-//                    the codes stand for, rounded once to bf16, a whole row per store instruction.
+// kv4_read_kernel    a block of 16 rows to shared memory in 16-byte pieces by 1, 2 or 4 warps, then 8 values a lane: the
+//                    numbers that the codes stand for, rounded once to bf16, whole rows to a store.
 //
 // Roundings are the bf16 model's (norm and each step of the rotation round to bf16), so a cached key is the 4-bit form
 // of the row the bf16 cache would hold. The norm's sum of squares and its root are taken in 64 bits: products of two
@@ -693,74 +693,82 @@ __global__ void __launch_bounds__(256, 4)
   }
 }
 
-constexpr int kReadWarps = 4;
+// hd / 64 warps take a block, four rows of 256 values (or as many of shorter rows) each; a CTA 4 warps, 256 / hd blocks. So a
+// lane has 8 values whatever the head size. Bound by the bytes, nearly all of them the bf16 rows written: B200, 65536 rows
+// of 1024 values (4 x 256, 8 x 128, 16 x 64) 58 us of 54 (353 MB at the measured 6.55 TB/s), 16384 rows 16 us of 13.5; a
+// warp a block with hd / 32 values a lane took 59, 66 and 81 us.
+template <int HD>
+struct ReadPlan {
+  static constexpr int WARPS = 4, PER_BLOCK = HD / 64, BLOCKS = WARPS / PER_BLOCK;
+};
 
 template <int HD>
-__global__ void __launch_bounds__(kReadWarps * 32) kv4_read_kernel(const __grid_constant__ Kv4ReadArgs a, int r0,
-                                                                   int spans, long tasks) {
+__global__ void __launch_bounds__(ReadPlan<HD>::WARPS * 32)
+    kv4_read_kernel(const __grid_constant__ Kv4ReadArgs a, int r0, int spans, long tasks) {
   using L = Kv4L<HD>;
-  constexpr int PER = L::PER, LANES = 32 / PER, PIECES = L::BYTES / 16;
-  __shared__ uint4 held[kReadWarps][PIECES];
+  using P = ReadPlan<HD>;
+  constexpr int PIECES = L::BYTES / 16, STEP = 32 * P::PER_BLOCK;
+  constexpr int LANES = HD / 8, ROWS = 32 / LANES;   // lanes of a row, rows of a warp's step
+  __shared__ uint4 held[P::BLOCKS][PIECES];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long task = (long)blockIdx.x * kReadWarps + warp;
-  if (task >= tasks) return;
-  const int x = (int)(task % spans);
-  const int gs = (int)(task / spans), g = gs % a.c.hkv, sq = gs / a.c.hkv;
-  const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
-  // rows [lo, hi) of the block, in rows of the output behind t0
-  const int block0 = first < 0 ? 0 : first / 16;
-  const int t0 = (int)((long)(block0 + x) * 16 - (first < 0 ? 0 : first));   // output row of the block's row 0
-  const int lo = max(0, -t0), hi = min(16, a.n - t0);
-  if (lo >= hi) return;
-  const long row = (long)(block0 + x) * 16;
-  const uint8_t* block = first >= 0 && row < a.c.rows[sq] ? kv4_block<HD>(a.c, sq, g, (int)row) : nullptr;
-  const long at = (long)(r0 + sq) * a.out_seq + (long)g * a.out_head + (long)t0 * HD + lane * PER;
-  if (block == nullptr) {
-    if (first >= 0 && lane == 0) record_error(a.err, kErrBadIndex);
-    float zero[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) zero[j] = 0.f;
-    for (int r = lo; r < hi; ++r) {
-      kv4_store<PER>(a.k + at + (long)r * HD, zero);
-      kv4_store<PER>(a.v + at + (long)r * HD, zero);
+  const int mine = warp / P::PER_BLOCK, part = warp % P::PER_BLOCK;
+  const long task = (long)blockIdx.x * P::BLOCKS + mine;
+  int lo = 0, hi = 0, t0 = 0, g = 0, sq = 0;         // rows [lo, hi) of the block, in rows of the output behind t0
+  const uint8_t* block = nullptr;
+  if (task < tasks) {
+    const int x = (int)(task % spans), gs = (int)(task / spans);
+    g = gs % a.c.hkv, sq = gs / a.c.hkv;
+    const int first = a.row0 != nullptr ? __ldg(a.row0 + r0 + sq) : a.row0_host;
+    const long row = first < 0 ? 16l * x : (long)(first / 16 + x) * 16;
+    t0 = (int)(row - (first < 0 ? 0 : first));
+    lo = max(0, -t0), hi = min(16, a.n - t0);
+    if (lo < hi && first >= 0) {
+      if (row < a.c.rows[sq]) block = kv4_block<HD>(a.c, sq, g, (int)row);
+      if (block == nullptr && part == 0 && lane == 0) record_error(a.err, kErrBadIndex);
     }
-    return;
   }
+  if (block != nullptr) {
 #pragma unroll
-  for (int j = 0; j < (PIECES + 31) / 32; ++j)
-    if (lane + 32 * j < PIECES) held[warp][lane + 32 * j] = __ldg(reinterpret_cast<const uint4*>(block) + lane + 32 * j);
-  __syncwarp();
-  const uint8_t* b = reinterpret_cast<const uint8_t*>(held[warp]);
-  const int i = lane / LANES, in = lane % LANES;
-#pragma unroll 4
-  for (int r = lo; r < hi; ++r) {
-    uint32_t c[2];
-    if constexpr (PER == 8) {
-      c[0] = *reinterpret_cast<const uint32_t*>(b + L::k_word(r, in, i));
-      c[1] = *reinterpret_cast<const uint16_t*>(b + L::v_chunk(r, 2 * in) + 2 * i) |
-             (uint32_t)*reinterpret_cast<const uint16_t*>(b + L::v_chunk(r, 2 * in + 1) + 2 * i) << 16;
-    } else if constexpr (PER == 4) {
-      c[0] = *reinterpret_cast<const uint16_t*>(b + L::k_word(r, in / 2, i) + 2 * (in & 1));
-      c[1] = *reinterpret_cast<const uint16_t*>(b + L::v_chunk(r, in) + 2 * i);
-    } else {
-      c[0] = b[L::k_word(r, in / 4, i) + (in & 3)];
-      c[1] = b[L::v_chunk(r, in / 2) + 2 * i + (in & 1)];
+    for (int j = 0; j < (PIECES + STEP - 1) / STEP; ++j) {
+      const int piece = part * 32 + lane + j * STEP;
+      if (piece < PIECES) held[mine][piece] = __ldg(reinterpret_cast<const uint4*>(block) + piece);
     }
-    const int at_s[2] = {r * L::NG + i, i * 16 + kv4_slot(r)};
+  }
+  __syncthreads();
+  const uint8_t* b = reinterpret_cast<const uint8_t*>(held[mine]);
+  const int j = lane % LANES, i = j / 4, in = j % 4;
+  const long at = (long)(r0 + sq) * a.out_seq + (long)g * a.out_head + (long)t0 * HD + 8 * j;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const float s = __half2float(reinterpret_cast<const __half*>(b + (x ? L::VS : L::KS))[at_s[x]]);
-      const float m = __half2float(reinterpret_cast<const __half*>(b + (x ? L::VM : L::KM))[at_s[x]]);
-      const float size = kv4_size(b[(x ? L::VE : L::KE) + r]);
-      float v[PER];
+  for (int y = 0; y < 4; ++y) {
+    const int r = (4 * part + y) * ROWS + lane / LANES;
+    if (r < lo || r >= hi) continue;
+    uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (block != nullptr) {
+      const uint32_t c[2] = {*reinterpret_cast<const uint32_t*>(b + L::k_word(r, in, i)),
+                             *reinterpret_cast<const uint16_t*>(b + L::v_chunk(r, 2 * in) + 2 * i) |
+                                 (uint32_t)*reinterpret_cast<const uint16_t*>(b + L::v_chunk(r, 2 * in + 1) + 2 * i) << 16};
+      const int at_s[2] = {r * L::NG + i, i * 16 + kv4_slot(r)};
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        // the code as a number: 2^23 + c minus 2^23
-        const float f = __int_as_float(0x4b000000 | (c[x] >> (4 * j) & 15)) - 8388608.f;
-        v[j] = size * fmaf(s, f, m);
+      for (int x = 0; x < 2; ++x) {
+        const Two s(__half2float(reinterpret_cast<const __half*>(b + (x ? L::VS : L::KS))[at_s[x]]));
+        const Two m(__half2float(reinterpret_cast<const __half*>(b + (x ? L::VM : L::KM))[at_s[x]]));
+        const Two size(kv4_size(b[(x ? L::VE : L::KE) + r]));
+        // the codes as numbers: 2^23 + c, put together from bytes, minus 2^23
+        const uint32_t even = c[x] & 0x0f0f0f0fu, odd = c[x] >> 4 & 0x0f0f0f0fu;
+        uint32_t w[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const Two f(__uint_as_float(__byte_perm(even, 0x4b000000u, 0x7440 + z)),
+                      __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7440 + z)));
+          float v0, v1;
+          mul2(size, fma2(s, add2(f, Two(-8388608.f)), m)).get(v0, v1);
+          w[z] = pack_bf16x2(v0, v1);
+        }
+        out[x] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      kv4_store<PER>((x ? a.v : a.k) + at + (long)r * HD, v);
     }
+    *reinterpret_cast<uint4*>(a.k + at + (long)r * HD) = out[0];
+    *reinterpret_cast<uint4*>(a.v + at + (long)r * HD) = out[1];
   }
 }
 
@@ -806,6 +814,13 @@ void launch_append(Kv4AppendArgs a, int r0, int seqs, cudaStream_t stream) {
   count_launch();
 }
 
+template <int HD>
+void launch_read(const Kv4ReadArgs& a, int r0, int spans, long tasks, cudaStream_t stream) {
+  using P = ReadPlan<HD>;
+  const unsigned ctas = (unsigned)((tasks + P::BLOCKS - 1) / P::BLOCKS);
+  kv4_read_kernel<HD><<<ctas, P::WARPS * 32, 0, stream>>>(a, r0, spans, tasks);
+}
+
 }  // namespace
 
 void kv4_append(const Kv4AppendArgs& a, int r0, int seqs, cudaStream_t stream) {
@@ -823,11 +838,10 @@ void kv4_read(const Kv4ReadArgs& a, int r0, int seqs, cudaStream_t stream) {
   const int spans = a.row0 == nullptr ? (a.row0_host + a.n - 1) / 16 - a.row0_host / 16 + 1 : (a.n + 14) / 16 + 1;
   const long tasks = (long)seqs * spans * a.c.hkv;
   if (tasks <= 0 || a.n <= 0) return;
-  const unsigned blocks = (unsigned)((tasks + kReadWarps - 1) / kReadWarps);
   switch (a.c.hd) {
-    case 64: kv4_read_kernel<64><<<blocks, kReadWarps * 32, 0, stream>>>(a, r0, spans, tasks); break;
-    case 128: kv4_read_kernel<128><<<blocks, kReadWarps * 32, 0, stream>>>(a, r0, spans, tasks); break;
-    case 256: kv4_read_kernel<256><<<blocks, kReadWarps * 32, 0, stream>>>(a, r0, spans, tasks); break;
+    case 64: launch_read<64>(a, r0, spans, tasks, stream); break;
+    case 128: launch_read<128>(a, r0, spans, tasks, stream); break;
+    case 256: launch_read<256>(a, r0, spans, tasks, stream); break;
     default: throw std::runtime_error("kv4_read: head_dim 64 / 128 / 256");
   }
   count_launch();
