@@ -55,8 +55,6 @@ __host__ __device__ constexpr int kv4_slot(int r) { return 4 * ((r & 7) >> 1) + 
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-__device__ __forceinline__ float kv4_bfr(float x) { return __bfloat162float(__float2bfloat16(x)); }
-
 __device__ __forceinline__ float kv4_pow2(int e) { return __int_as_float((e + 127) << 23); }
 
 // 2^e of an exponent byte, NaN for a marked row
@@ -73,31 +71,12 @@ __device__ __forceinline__ uint8_t* kv4_block(const Kv4Pages& c, int sq, int g, 
   return c.pool + slab * Kv4L<HD>::BYTES;
 }
 
-template <int PER>
-__device__ __forceinline__ void kv4_load(const __nv_bfloat16* p, float (&v)[PER]) {
-  if constexpr (PER == 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
-  } else if constexpr (PER == 4) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    v[0] = bf16_lo(u.x), v[1] = bf16_hi(u.x), v[2] = bf16_lo(u.y), v[3] = bf16_hi(u.y);
-  } else {
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-    v[0] = bf16_lo(u), v[1] = bf16_hi(u);
-  }
+__device__ __forceinline__ void kv4_load(const __nv_bfloat16* p, float (&v)[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  v[0] = bf16_lo(u.x), v[1] = bf16_hi(u.x), v[2] = bf16_lo(u.y), v[3] = bf16_hi(u.y);
 }
-
-template <int PER>
-__device__ __forceinline__ void kv4_store(__nv_bfloat16* p, const float (&v)[PER]) {
-  if constexpr (PER == 8)
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                              pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-  else if constexpr (PER == 4)
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-  else
-    *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(v[0], v[1]);
+__device__ __forceinline__ void kv4_store(__nv_bfloat16* p, const float (&v)[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
 }  // namespace rf

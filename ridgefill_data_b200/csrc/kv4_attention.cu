@@ -112,12 +112,12 @@ __device__ __forceinline__ void finish(const Kv4AttnArgs& a, int r, int col, int
   float g[4] = {n, n, n, n};
   if (a.gate != nullptr) {
     float z[4];
-    kv4_load<4>(a.gate + (long)r * a.gate_row + (long)h * a.gate_head + e, z);
+    kv4_load(a.gate + (long)r * a.gate_row + (long)h * a.gate_head + e, z);
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[j] = n / (1.f + __expf(-z[j]));
   }
   const float v[4] = {o.x * g[0], o.y * g[1], o.z * g[2], o.w * g[3]};
-  kv4_store<4>(a.out + (long)r * a.out_row + col, v);
+  kv4_store(a.out + (long)r * a.out_row + col, v);
 }
 
 constexpr float kTop = 14.f;    // P <= 2^14
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
     if (s > 0) return;
     if (p >= 0 && g == 0 && threadIdx.x == 0) record_error(a.err, kErrBadIndex);
     for (int x = threadIdx.x; x < G * HD / 4; x += kWarps * 32)
-      kv4_store<4>(a.out + (long)r * a.out_row + g * G * HD + 4 * x, {0.f, 0.f, 0.f, 0.f});
+      kv4_store(a.out + (long)r * a.out_row + g * G * HD + 4 * x, {0.f, 0.f, 0.f, 0.f});
     return;
   }
   const int keys = split_keys(p, a.most), start = s * keys;
