@@ -7,10 +7,10 @@
 // kv4_combine_kernel  grid (query head, sequence): the splits' partials in a fixed order, the sum's division, the gate. Both
 //                     start while the kernel before them ends.
 //
-// Bound by the cache's bytes: inside a CTA's loop DRAM runs at its rate, and what is above the floor is the CTAs' start (2 us:
-// position, page ids, query) and join (1.6 us), which the CTAs that share an SM reach together. B200: four streams behind
-// 128K rows of 8 heads of 128 130 us (680 MB: 104 at the measured 6.55 TB/s), eight behind up to 32K rows of 4 heads of 256
-// 46 us (190 MB: 29), one behind 16K rows of those 13 us (21 MB: 3.2; latency: 8 blocks a warp, one after another).
+// Bound by the cache's bytes: inside a CTA's loop DRAM runs at its rate, and what is above the floor is the CTAs' start (3 us:
+// position, page ids, query, first block) and join (1.6 us), which the CTAs that share an SM reach together. B200: four streams behind
+// 128K rows of 8 heads of 128 132 us (680 MB: 104 at the measured 6.55 TB/s), eight behind up to 32K rows of 4 heads of 256
+// 47 us (190 MB: 29), one behind 16K rows of those 14 to 16 us (21 MB: 3.2; latency: 8 blocks a warp, one after another).
 //
 // Both products run on the tensor cores with the cache as the A operand (16 rows) and the G <= 8 query heads as its 8
 // columns, so nothing of a tile is wasted on absent query rows, and with the codes as they are stored: a masked nibble
