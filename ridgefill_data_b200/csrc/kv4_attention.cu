@@ -20,8 +20,9 @@
 //   O   = 2^24 sum_j C_j (P_j s_ji) + sum_j m_ji P_j
 // per 32-dim group i: one fp32 FMA a score and group on the K side, one fp16 multiply of P on the V side. The m sums are
 // one more product each (Q_i as two fp16 halves of 22 bits together). P takes the V row's size 2^e_j on the way, so
-// the running maximum is over S_j + e_j and P and P s stay inside fp16 whatever the rows' sizes; P is at most 2^14,
-// and the maximum is raised only when a score would pass that.
+// the running maximum is over S_j + e_j and P and P s stay inside fp16 whatever the rows' sizes (fit_sizes sees to the rows
+// whose stored exponent is not their size); P is at most 2^14, and the maximum is raised only when a score would pass
+// that.
 #include "kv4.cuh"
 
 #include "kernels.h"
@@ -399,6 +400,52 @@ struct Warp {
   }
 };
 
+// A V row's exponent byte states its size but for rows of 2^41 and more, whose exponent the cache holds to 40: their z
+// reaches 2^16 and their step 2^13.1, past what P leaves in fp16. Such rows are brought to z below 2 in the ring, exponent
+// and all, before their block is used: s and m by a power of two (exact, or to 2^-25 of a row of size 1), so that in every
+// block P s <= 2^14 (4 / 15) and l, in units of 2^-e, stays above 2^-56.
+template <int HD>
+__device__ __forceinline__ bool size_misfits(const uint8_t* block, int r) {
+  return block[Kv4L<HD>::VE + r] == 127 + kKv4Limit;
+}
+
+template <int HD>
+__device__ __forceinline__ void fit_size(uint8_t* block, int r) {
+  using L = Kv4L<HD>;
+  __half* s = reinterpret_cast<__half*>(block + L::VS) + kv4_slot(r);
+  __half* m = reinterpret_cast<__half*>(block + L::VM) + kv4_slot(r);
+  float top = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < L::NG; ++i) {
+    const float low = __half2float(m[16 * i]), high = fmaf(15.f, __half2float(s[16 * i]), low);
+    top = fmaxf(top, fmaxf(fabsf(low), fabsf(high)));
+  }
+  const int byte = block[L::VE + r];
+  if (byte == 127 + kKv4Limit && top >= 2.f) {
+    const int up = min((__float_as_int(top) >> 23) - 127, 16);
+    const float down = kv4_pow2(-up);
+#pragma unroll 1
+    for (int i = 0; i < L::NG; ++i) {
+      s[16 * i] = __float2half_rn(__half2float(s[16 * i]) * down);
+      m[16 * i] = __float2half_rn(__half2float(m[16 * i]) * down);
+    }
+    block[L::VE + r] = (uint8_t)(byte + up);
+  }
+}
+
+// every row of NB blocks in the ring; the next copy into them comes after the fence
+template <int HD, int NB>
+__device__ __forceinline__ void fit_sizes(uint8_t* b, int lane) {
+  uint8_t* block = b + (lane >> 4) * Kv4L<HD>::BYTES;
+  const bool misfit = lane < 16 * NB && size_misfits<HD>(block, lane & 15);
+  if (!__any_sync(kFull, misfit)) return;
+  if (misfit) {
+    fit_size<HD>(block, lane & 15);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncwarp();
+}
+
 // Two blocks a step where the registers allow (hd 64, 128: 147 -> 130 us for four streams behind 128K rows; a second chain
 // of dependent instructions beside the first); at hd 256 one, with the query's fragments left in shared memory for 3 CTAs
 // an SM. The ring holds what 12 to 24 warps an SM keep in flight: 124 to 185 KB.
@@ -488,7 +535,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
       }
       break;
     }
-    const uint8_t* b = ring + stage * NB * L::BYTES;
+    uint8_t* b = ring + stage * NB * L::BYTES;
+    fit_sizes<HD, NB>(b, lane);
     const unsigned loaded = __ballot_sync(kFull, good) >> (stage * NB);
     int live[NB];
     bool full = true;

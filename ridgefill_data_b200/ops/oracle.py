@@ -271,6 +271,15 @@ def kv4_values(byte, s, m, c):
     return torch.where((byte == KV4_MARK)[..., None], torch.full_like(v, math.nan), v)
 
 
+def kv4_fitted(byte, s, m):
+    """(byte, s, m) of quantised V rows as attention uses them: a row of 2^41 and more, whose exponent the cache holds to 40,
+    with its own exponent and its z below 2."""
+    top = torch.maximum(m.abs(), (m + 15 * s).abs()).amax(-1)
+    up = torch.where((byte == 167) & (top >= 2), torch.frexp(top)[1] - 1, 0).clamp(0, 16)
+    down = torch.pow(2.0, -up.double()).float()[..., None]
+    return byte + up, (s * down).half().float(), (m * down).half().float()
+
+
 def kv4_places(hd, row):
     """Where row `row` (0 .. 15) of a block keeps its parts: the 4-bit steps of K's and V's codes [hd] from the block's
     start, and the bytes of K's s and m [hd / 32], V's s and m, K's and V's exponent."""
