@@ -273,8 +273,7 @@ __device__ __forceinline__ void put_row(const Row<HD / 32>& row, uint8_t* block,
   for (int j = 0; j < PER / 2; ++j) top = __vmaxu2(top, row.w[j] & 0x7fff7fffu);
   top = __reduce_max_sync(kFull, max(top & 0xffffu, top >> 16));
   const bool bad = top >= 0x5b80u;   // 2^56 and above, infinities and NaN
-  int e = top == 0 ? 0 : (int)(top >> 7) - 127;
-  e = max(-kKv4Limit, min(kKv4Limit, e));
+  const int e = max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
   Row<PER> v = row;
   if (bad)
 #pragma unroll
@@ -546,7 +545,7 @@ __device__ __forceinline__ void put_heads(uint32_t (&v)[8], uint8_t* block, bool
 #pragma unroll
     for (int x = 0; x < 8; ++x) v[x] = 0;
   }
-  const int e = top == 0 ? 0 : max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
+  const int e = max(-kKv4Limit, min(kKv4Limit, (int)(top >> 7) - 127));
   const Steps st(fminf(bf16_lo(least), bf16_hi(least)), fmaxf(bf16_lo(most), bf16_hi(most)), kv4_pow2(-e));
   uint32_t codes[2];
   st.codes<16>(v, codes);

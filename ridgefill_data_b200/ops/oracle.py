@@ -254,7 +254,8 @@ def kv4_quantise(y):
     y = y.float()
     top = y.abs().amax(-1)
     bad = ~(top < 2.0 ** 56)
-    e = (torch.frexp(torch.where(bad | (top == 0), torch.ones_like(top), top))[1] - 1).clamp(-40, 40)
+    e = (torch.frexp(torch.where(bad, torch.ones_like(top), top))[1] - 1).clamp(-40, 40)
+    e = torch.where(top == 0, torch.full_like(e, -40), e)
     z = torch.where(bad[..., None], torch.zeros_like(y), y) * torch.pow(2.0, -e.double()).float()[..., None]
     z = z.unflatten(-1, (-1, 32))
     low, high = z.amin(-1), z.amax(-1)

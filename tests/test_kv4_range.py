@@ -28,3 +28,11 @@ def test_probability_times_step_stays_inside_fp16(exponent):
     was, now = ops.kv4_values(byte, s, m, c), ops.kv4_values(*fit, c)
     assert ((was - now).abs() <= 16 * 2.0 ** -25 * torch.pow(2.0, fit[0].double() - 127)[:, None]).all()
     assert torch.equal(was, now) or exponent > 40
+
+
+def test_a_row_of_zeros_has_the_smallest_size():
+    """Beside rows of any size a row of zeros does not raise the running maximum (over score + exponent byte)."""
+    y = torch.zeros(4, 64)
+    y[1], y[2, 3], y[3, 40] = -0.0, 2.0 ** -40, -(2.0 ** -30)
+    byte, _, _ = ops.kv4_fitted(*ops.kv4_quantise(y.bfloat16())[:3])
+    assert byte.tolist() == [87, 87, 87, 97]

@@ -65,3 +65,24 @@ def test_the_largest_value_rows(hd):
     for last in (0, 6, 7, 19):
         pos = torch.tensor([last], dtype=torch.int32, device=DEV)
         _check(kv4.attention(q, pool, table, pos, 0.1), _reference(q, pool, [table], pos, 0.1))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("size", [-10, -22, -28, -34, -38])
+@pytest.mark.parametrize("zeros", [[0], [99], list(range(20, 50))], ids=["first", "last", "many"])
+def test_zero_value_rows_beside_small_ones(hd, size, zeros):
+    """V rows of zeros take their weight and nothing else: what rows of any size add keeps its bits. First among rows of
+    similar scores, then with 2^13 times the weight of the others."""
+    n = 100
+    k, v = _rows(n, 2, hd, seed=7), _rows(n, 2, hd, seed=8) * 2.0 ** size
+    v[zeros] = 0.0
+    q = _rows(1, 4, hd, seed=9).bfloat16()
+    pos = torch.tensor([n - 1], dtype=torch.int32, device=DEV)
+    for lead in (0.0, 13 * 0.6931):
+        k[zeros] = 0.0
+        if lead:                               # the zero rows' keys along the first query of each KV head: score + lead
+            q[0, 1::2] = q[0, ::2]
+            w = q[0, ::2].float()
+            k[zeros] = w / w.square().sum(-1, keepdim=True) * lead / 0.1
+        pool, table = _cache(k, v)
+        _check(kv4.attention(q, pool, table, pos, 0.1), _reference(q, pool, [table], pos, 0.1))
