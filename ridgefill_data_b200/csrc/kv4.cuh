@@ -4,7 +4,7 @@
 //   e   exponent, max|y| in [2^e, 2^(e+1)), held to -40 .. 40 (-40 for a row of zeros): 2^-e and products with it stay
 //       inside fp32. Rows of 2^41 and more have z up to 2^16, rows below 2^-40 have z below 1: m and s stay inside fp16.
 //       Byte e + 127; 255 marks a row with a non-finite value or one of 2^56 or more: its values are NaN (its codes and
-//       scales are zeros, so a masked one adds exactly nothing).
+//       scales are zeros, so a masked one adds exactly nothing). Zero bytes, a new pool's, stand for zeros.
 //   m, s  per 32 dims of z = y 2^-e: fp16(min z) and fp16((max z - min z) / 15)
 //   c   per value: round((z - m) / s) in 0 .. 15; the value it stands for is 2^e (m + s c)
 // that is 1.25 hd + 2 bytes for K and V together, against 4 hd in bf16.

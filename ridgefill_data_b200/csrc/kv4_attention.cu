@@ -20,7 +20,7 @@
 //   O   = 2^24 sum_j C_j (P_j s_ji) + sum_j m_ji P_j
 // per 32-dim group i: one fp32 FMA a score and group on the K side, one fp16 multiply of P on the V side. The m sums are
 // one more product each (Q_i as two fp16 halves of 22 bits together). P takes the V row's size 2^e_j on the way, so
-// the running maximum is over S_j + e_j and P and P s stay inside fp16 whatever the rows' sizes (fit_sizes sees to the rows
+// the running maximum is over S_j + e_j and P and P s stay inside fp16 whatever the rows' sizes (fit_size sees to the rows
 // whose stored exponent is not their size); P is at most 2^14, and the maximum is raised only when a score would pass
 // that.
 #include "kv4.cuh"
@@ -200,6 +200,41 @@ struct QueryLoad {
   }
 };
 
+// A V row's exponent byte states its size but for
+//   rows of 2^41 and more, whose exponent the cache holds to 40: their z reaches 2^16 and their step 2^13.1, past what P
+//   leaves in fp16;
+//   rows that nothing was appended to, zeros under the new pool's zero byte: l, in units of 2^-e, would overflow.
+// Such rows get their own size in the ring before their block's values are used: large ones z below 2, s and m by a power
+// of two (exact, or to 2^-25 of a row of size 1), zeros the smallest size. So in every block P s <= 2^14 (4 / 15), and l
+// lies between 2^-56 and 2^54 a key. A marked row (255) misfits too and is left as it is.
+__device__ __forceinline__ bool size_misfits(int byte) { return (unsigned)(byte - (127 - kKv4Limit)) >= 2u * kKv4Limit; }
+
+template <int HD>
+__device__ __forceinline__ void fit_size(uint8_t* block, int r) {
+  using L = Kv4L<HD>;
+  __half* s = reinterpret_cast<__half*>(block + L::VS) + kv4_slot(r);
+  __half* m = reinterpret_cast<__half*>(block + L::VM) + kv4_slot(r);
+  float top = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < L::NG; ++i) {
+    const float low = __half2float(m[16 * i]), high = fmaf(15.f, __half2float(s[16 * i]), low);
+    top = fmaxf(top, fmaxf(fabsf(low), fabsf(high)));
+  }
+  const int byte = block[L::VE + r];
+  if (top == 0.f && byte < 127 - kKv4Limit) block[L::VE + r] = 127 - kKv4Limit;
+  if (byte == 127 + kKv4Limit && top >= 2.f) {
+    const int up = min((__float_as_int(top) >> 23) - 127, 16);
+    const float down = kv4_pow2(-up);
+#pragma unroll 1
+    for (int i = 0; i < L::NG; ++i) {
+      s[16 * i] = __float2half_rn(__half2float(s[16 * i]) * down);
+      m[16 * i] = __float2half_rn(__half2float(m[16 * i]) * down);
+    }
+    block[L::VE + r] = (uint8_t)(byte + up);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the next copy into the ring
+}
+
 // The state of a warp over its keys. Fragment layouts as in mma.cuh: lane (g, t) = (lane / 4, lane % 4).
 template <int HD>
 struct Warp {
@@ -248,8 +283,9 @@ struct Warp {
 
   // NB blocks of 16 keys at b; LAST: only the first live[u] rows of block u exist (the others' bytes may be anything)
   template <bool LAST, int NB>
-  __device__ __forceinline__ void blocks(const uint8_t* b, const int (&live)[NB], int lane) {
+  __device__ __forceinline__ void blocks(uint8_t* b, const int (&live)[NB], int lane) {
     const int g = lane >> 2, t = lane & 3;
+    bool misfit = false;
     // scores: rows g and g + 8, columns 2t and 2t + 1; y = score + size of the V row (its byte)
     constexpr int KW = NG < 4 ? NG : 4;    // words of one load
     float y[NB][4], iv[NB][2];
@@ -302,6 +338,7 @@ struct Warp {
         const int ve = k[L::VE + g + 8 * r];
         const float kz = __int_as_float(k[L::KE + g + 8 * r] << 23), e = (float)ve;
         iv[u][r] = __int_as_float((254 - ve) << 23);
+        misfit |= size_misfits(ve);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
           y[u][2 * r + c] = fmaf(fmaf(s[2 * r + c], 16777216.f, cm[2 * r + c]), kz * cs[c], e);
@@ -309,13 +346,35 @@ struct Warp {
       }
     }
     float top[2];
+    auto find_top = [&] {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      top[c] = fmaxf(y[0][c], y[0][c + 2]);
+      for (int c = 0; c < 2; ++c) {
+        top[c] = fmaxf(y[0][c], y[0][c + 2]);
 #pragma unroll
-      for (int u = 1; u < NB; ++u) top[c] = fmaxf(top[c], fmaxf(y[u][c], y[u][c + 2]));
-    }
-    if (__any_sync(kFull, top[0] > ref[0] + kTop || top[1] > ref[1] + kTop)) {
+        for (int u = 1; u < NB; ++u) top[c] = fmaxf(top[c], fmaxf(y[u][c], y[u][c + 2]));
+      }
+    };
+    find_top();
+    if (__any_sync(kFull, misfit || top[0] > ref[0] + kTop || top[1] > ref[1] + kTop)) {
+      if (__any_sync(kFull, misfit)) {
+        float was[NB][2];
+#pragma unroll
+        for (int u = 0; u < NB; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) was[u][r] = (float)b[u * L::BYTES + L::VE + g + 8 * r];
+        __syncwarp();
+        if (lane < 16 * NB) fit_size<HD>(b + (lane >> 4) * L::BYTES, lane & 15);
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < NB; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int ve = b[u * L::BYTES + L::VE + g + 8 * r];
+            y[u][2 * r] += (float)ve - was[u][r], y[u][2 * r + 1] += (float)ve - was[u][r];
+            if (iv[u][r] != 0.f) iv[u][r] = __int_as_float((254 - ve) << 23);
+          }
+        find_top();
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float m = top[c];
@@ -399,52 +458,6 @@ struct Warp {
       }
   }
 };
-
-// A V row's exponent byte states its size but for rows of 2^41 and more, whose exponent the cache holds to 40: their z
-// reaches 2^16 and their step 2^13.1, past what P leaves in fp16. Such rows are brought to z below 2 in the ring, exponent
-// and all, before their block is used: s and m by a power of two (exact, or to 2^-25 of a row of size 1), so that in every
-// block P s <= 2^14 (4 / 15) and l, in units of 2^-e, stays above 2^-56.
-template <int HD>
-__device__ __forceinline__ bool size_misfits(const uint8_t* block, int r) {
-  return block[Kv4L<HD>::VE + r] == 127 + kKv4Limit;
-}
-
-template <int HD>
-__device__ __forceinline__ void fit_size(uint8_t* block, int r) {
-  using L = Kv4L<HD>;
-  __half* s = reinterpret_cast<__half*>(block + L::VS) + kv4_slot(r);
-  __half* m = reinterpret_cast<__half*>(block + L::VM) + kv4_slot(r);
-  float top = 0.f;
-#pragma unroll 1
-  for (int i = 0; i < L::NG; ++i) {
-    const float low = __half2float(m[16 * i]), high = fmaf(15.f, __half2float(s[16 * i]), low);
-    top = fmaxf(top, fmaxf(fabsf(low), fabsf(high)));
-  }
-  const int byte = block[L::VE + r];
-  if (byte == 127 + kKv4Limit && top >= 2.f) {
-    const int up = min((__float_as_int(top) >> 23) - 127, 16);
-    const float down = kv4_pow2(-up);
-#pragma unroll 1
-    for (int i = 0; i < L::NG; ++i) {
-      s[16 * i] = __float2half_rn(__half2float(s[16 * i]) * down);
-      m[16 * i] = __float2half_rn(__half2float(m[16 * i]) * down);
-    }
-    block[L::VE + r] = (uint8_t)(byte + up);
-  }
-}
-
-// every row of NB blocks in the ring; the next copy into them comes after the fence
-template <int HD, int NB>
-__device__ __forceinline__ void fit_sizes(uint8_t* b, int lane) {
-  uint8_t* block = b + (lane >> 4) * Kv4L<HD>::BYTES;
-  const bool misfit = lane < 16 * NB && size_misfits<HD>(block, lane & 15);
-  if (!__any_sync(kFull, misfit)) return;
-  if (misfit) {
-    fit_size<HD>(block, lane & 15);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-  __syncwarp();
-}
 
 // Two blocks a step where the registers allow (hd 64, 128: 147 -> 130 us for four streams behind 128K rows; a second chain
 // of dependent instructions beside the first); at hd 256 one, with the query's fragments left in shared memory for 3 CTAs
@@ -536,7 +549,6 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
       break;
     }
     uint8_t* b = ring + stage * NB * L::BYTES;
-    fit_sizes<HD, NB>(b, lane);
     const unsigned loaded = __ballot_sync(kFull, good) >> (stage * NB);
     int live[NB];
     bool full = true;

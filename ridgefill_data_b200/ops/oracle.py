@@ -274,11 +274,12 @@ def kv4_values(byte, s, m, c):
 
 def kv4_fitted(byte, s, m):
     """(byte, s, m) of quantised V rows as attention uses them: a row of 2^41 and more, whose exponent the cache holds to 40,
-    with its own exponent and its z below 2."""
+    with its own exponent and its z below 2; a row of the pool's first zero bytes with the smallest exponent."""
     top = torch.maximum(m.abs(), (m + 15 * s).abs()).amax(-1)
     up = torch.where((byte == 167) & (top >= 2), torch.frexp(top)[1] - 1, 0).clamp(0, 16)
     down = torch.pow(2.0, -up.double()).float()[..., None]
-    return byte + up, (s * down).half().float(), (m * down).half().float()
+    byte = torch.where((top == 0) & (byte < 87), torch.full_like(byte, 87), byte + up)
+    return byte, (s * down).half().float(), (m * down).half().float()
 
 
 def kv4_places(hd, row):

@@ -36,3 +36,5 @@ def test_a_row_of_zeros_has_the_smallest_size():
     y[1], y[2, 3], y[3, 40] = -0.0, 2.0 ** -40, -(2.0 ** -30)
     byte, _, _ = ops.kv4_fitted(*ops.kv4_quantise(y.bfloat16())[:3])
     assert byte.tolist() == [87, 87, 87, 97]
+    byte, s, m = ops.kv4_fitted(torch.tensor([0, 255]), torch.zeros(2, 2), torch.zeros(2, 2))
+    assert byte.tolist() == [87, 255] and not s.any() and not m.any()

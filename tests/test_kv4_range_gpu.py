@@ -86,3 +86,18 @@ def test_zero_value_rows_beside_small_ones(hd, size, zeros):
             k[zeros] = w / w.square().sum(-1, keepdim=True) * lead / 0.1
         pool, table = _cache(k, v)
         _check(kv4.attention(q, pool, table, pos, 0.1), _reference(q, pool, [table], pos, 0.1))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_rows_never_appended_are_zero_rows(hd):
+    """A pool starts zeroed: a visible row that nothing was appended to reads as zeros and counts as a row of zeros."""
+    pool, table = _cache(_rows(60, 2, hd, seed=1), _rows(60, 2, hd, seed=2) * 2.0 ** -20, page=96)
+    q = _rows(1, 6, hd, seed=3).bfloat16()
+    for last in (60, 95):
+        pos = torch.tensor([last], dtype=torch.int32, device=DEV)
+        _check(kv4.attention(q, pool, table, pos, 0.1), _reference(q, pool, [table], pos, 0.1))
+    empty = kv4.pool(8, 2, 96, hd)
+    table = torch.arange(8, dtype=torch.int32, device=DEV)
+    for last in (0, 95, 700):
+        pos = torch.tensor([last], dtype=torch.int32, device=DEV)
+        assert kv4.attention(q, empty, table, pos, 0.1).eq(0).all()
