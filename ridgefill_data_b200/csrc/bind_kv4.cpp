@@ -129,8 +129,8 @@ OptT kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
     for (const OptT* t : {&cos, &sin}) {
       need(**t, at::kBFloat16, c.pool, "RoPE table");
       TORCH_CHECK((*t)->dim() == 2 && (*t)->is_contiguous() && (*t)->size(1) == rot / 2 && aligned(**t) &&
-                      (*t)->size(0) == cos->size(0) && (*t)->size(0) < (1ll << 31),
-                  "kv4.append: RoPE tables [positions, rot / 2]");
+                      (*t)->size(0) == cos->size(0) && (*t)->size(0) < (1ll << 31) && (T == 0 || (*t)->size(0) > 0),
+                  "kv4.append: RoPE tables [positions, rot / 2] of one position or more");
     }
     a.cos = bf(*cos);
     a.sin = bf(*sin);
