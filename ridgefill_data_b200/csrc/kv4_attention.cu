@@ -528,10 +528,10 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<HD>::CTAS)
     mine += NB * kWarps * ST;
     page += step, in += left;
     if (in >= per) in -= per, ++page;
-    if (mine < blocks) id = __ldg(table + page);
+    if (mine < blocks) id = table[page];
   };
   __syncwarp();
-  if (lane < ST * NB && mine < blocks) id = __ldg(table + page);
+  if (lane < ST * NB && mine < blocks) id = table[page];
   QueryLoad<HD> loading;
   loading.load(a, a.q + (long)r * a.q_row + (long)g * G * a.q_head, G, warp, lane);
   if (lane < ST * NB && mine - lane % NB < blocks) issue();
