@@ -99,8 +99,9 @@ OptT kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
   const Cache c(pool, std::move(pages), "kv4.append");
   const int64_t R = (int64_t)c.pages.size();
   need(src, at::kBFloat16, c.pool, "src");
-  const int64_t qw = hq * c.hd * (gated ? 2 : 1);
-  TORCH_CHECK(src.dim() == 2 && src.stride(1) == 1 && hq >= 0 && hq + 2 * c.hkv <= 65535 &&
+  // each number's own range before a product or sum of it, which may pass 64 bits
+  const int64_t qw = hq >= 0 && hq <= 65535 ? hq * c.hd * (gated ? 2 : 1) : 0;
+  TORCH_CHECK(src.dim() == 2 && src.stride(1) == 1 && hq >= 0 && hq <= 65535 && hq + 2 * c.hkv <= 65535 &&
                   src.size(1) >= qw + 2 * (int64_t)c.hkv * c.hd,
               "kv4.append: rows [*, q heads | k heads | v heads], up to 65535 heads");
   TORCH_CHECK(aligned(src) && (src.size(0) <= 1 || src.stride(0) % 8 == 0) && small(src.stride(0)),
@@ -250,7 +251,7 @@ Tensor kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor po
   if (gate.has_value()) {
     need(*gate, at::kBFloat16, c.pool, "gate");
     TORCH_CHECK(gate->dim() == 2 && gate->size(0) == R && gate->stride(1) == 1 && gate_head >= 0 && gate_head % 8 == 0 &&
-                    gate->size(1) >= (hq - 1) * gate_head + c.hd && aligned(*gate) &&
+                    (hq == 1 || gate_head <= gate->size(1)) && gate->size(1) >= (hq - 1) * gate_head + c.hd && aligned(*gate) &&
                     (R <= 1 || gate->stride(0) % 8 == 0),
                 "kv4.attention: gate rows whose head h starts at column h * gate_head, 16-byte aligned");
     a.gate = bf(*gate);

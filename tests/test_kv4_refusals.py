@@ -22,3 +22,27 @@ def test_rope_tables_without_positions(T, where):
         kw["pos"] = torch.arange(T, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="RoPE tables|positions past"):
         kv4.append(src, pool, [table], **kw)
+
+
+@pytest.mark.parametrize("hq,gate_head", [(5, 2 ** 62), (3, 2 ** 63 - 8), (2, 2 ** 63 - 8), (5, 2 ** 61), (2, 520)])
+def test_gate_columns_past_the_row(hq, gate_head):
+    """The last head's gate would lie outside the row; (hq - 1) gate_head may pass 64 bits."""
+    pool, _, table = _args(hkv=1, hq=hq)
+    with pytest.raises(RuntimeError, match="gate rows"):
+        kv4.attention(torch.zeros(1, hq, 128).bfloat16(), pool, [table], torch.zeros(1, dtype=torch.int32), 0.1,
+                      gate=torch.zeros(1, 512).bfloat16(), gate_head=gate_head)
+
+
+@pytest.mark.parametrize("hq", [2 ** 63 - 1, 2 ** 62, 65536, -1])
+def test_query_heads_at_their_ends(hq):
+    pool, src, table = _args(T=0)
+    with pytest.raises(RuntimeError, match="up to 65535 heads"):
+        kv4.append(src, pool, [table], 0, q_heads=hq)
+
+
+def test_one_heads_gate_has_no_pitch():
+    """With one query head nothing is taken gate_head columns further."""
+    pool, _, table = _args(hkv=1, hq=1)
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        kv4.attention(torch.zeros(1, 1, 128).bfloat16(), pool, [table], torch.zeros(1, dtype=torch.int32), 0.1,
+                      gate=torch.zeros(1, 128).bfloat16(), gate_head=256)
