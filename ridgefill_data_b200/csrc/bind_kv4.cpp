@@ -1,7 +1,6 @@
 // Python bindings of the 4-bit K/V cache (kv4.h). Everything a kernel indexes by is checked here for type,
 // device, layout and extent; positions and page ids, which live in device memory, are checked by the kernels.
 #include <torch/extension.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -27,6 +26,33 @@ bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr())
 void need(const Tensor& t, at::ScalarType st, const Tensor& like, const char* name) {
   TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device().str(), ", the pool on ", like.device().str());
   TORCH_CHECK(t.scalar_type() == st, name, " has dtype ", t.scalar_type(), ", expected ", st);
+}
+
+// Whether some element of t lies `shift` elements behind another one of t (behind itself: not when `same`), dim after dim from
+// the widest stride, at the multiples that the inner dims (together `inner` elements wide at most) can make up for.
+bool meets(const Tensor& t, const std::vector<int64_t>& dims, size_t at, int64_t inner, int64_t shift, bool same) {
+  if (at == dims.size()) return shift == 0 && !same;
+  const int64_t stride = t.stride(dims[at]), last = t.size(dims[at]) - 1;   // last > 0
+  if (stride == 0) return true;
+  inner -= last * stride;
+  const auto down = [&](int64_t x) { return x >= 0 ? x / stride : -((-x + stride - 1) / stride); };
+  for (int64_t x = std::max(-last, -down(inner - shift)); x <= std::min(last, down(shift + inner)); ++x)
+    if (meets(t, dims, at + 1, inner, shift - x * stride, same && x == 0)) return true;
+  return false;
+}
+
+// Rows that a call writes into given outputs must share no element: t's own, or those of t and of a second output of t's
+// strides.
+void need_apart(const Tensor& t, const char* op, const OptT& second = c10::nullopt) {
+  if (t.numel() == 0) return;
+  std::vector<int64_t> dims;
+  int64_t inner = 0;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) dims.push_back(d), inner += (t.size(d) - 1) * t.stride(d);
+  std::sort(dims.begin(), dims.end(), [&](int64_t x, int64_t y) { return t.stride(x) > t.stride(y); });
+  const int64_t shift = second.has_value() ? ((const char*)second->data_ptr() - (const char*)t.data_ptr()) / t.element_size() : 0;
+  TORCH_CHECK(!meets(t, dims, 0, inner, shift, !second.has_value()), op,
+              ": an output's rows lie on each other (several of its elements at one memory location)");
 }
 
 // pool and page tables of every sequence -> the launch's part of them
@@ -150,13 +176,14 @@ OptT kv4_append(Tensor src, Tensor pool, std::vector<Tensor> pages, OptT row0, i
                 "kv4.append: positions past the RoPE tables' ", std::to_string(a.table_rows));
   if (hq == 0) q_out = c10::nullopt;
   if (hq > 0) {
-    if (!q_out.has_value()) q_out = at::empty({src.size(0), hq, c.hd}, src.options());
+    const bool given = q_out.has_value();
+    if (!given) q_out = at::empty({src.size(0), hq, c.hd}, src.options());
     need(*q_out, at::kBFloat16, c.pool, "q_out");
     TORCH_CHECK(q_out->dim() == 3 && q_out->size(0) == src.size(0) && q_out->size(1) == hq && q_out->size(2) == c.hd &&
                     q_out->stride(2) == 1 && small(q_out->stride(0)) && small(q_out->stride(1)) &&
                     q_out->stride(0) % 8 == 0 && q_out->stride(1) % 8 == 0 && aligned(*q_out),
                 "kv4.append: q_out [rows, q heads, head_dim], 16-byte aligned");
-    at::assert_no_internal_overlap(*q_out);
+    if (given) need_apart(*q_out, "kv4.append");
     a.q_out = bf(*q_out);
     a.q_out_row = (int)q_out->stride(0);
     a.q_out_head = (int)q_out->stride(1);
@@ -204,8 +231,9 @@ std::tuple<Tensor, Tensor> kv4_read(Tensor pool, std::vector<Tensor> pages, OptT
     TORCH_CHECK(t->numel() == 0 || (t->stride(3 - lead) == 1 && t->stride(2 - lead) == c.hd && t->stride(1 - lead) % 8 == 0 &&
                                     (single || t->stride(0) % 8 == 0) && t->strides() == k.strides() && aligned(*t)),
                 "kv4.read: k and v rows head_dim apart, 16-byte aligned, the same strides");
-    at::assert_no_internal_overlap(*t);
+    if (k_out.has_value()) need_apart(*t, "kv4.read");
   }
+  if (k_out.has_value()) need_apart(k, "kv4.read", v);
   rf::Kv4ReadArgs a{};
   if (R == 0) return {k, v};
   a.row0 = first_rows(row0, row0_host, c, n, "kv4.read");
@@ -246,7 +274,7 @@ Tensor kv4_attention(Tensor q, Tensor pool, std::vector<Tensor> pages, Tensor po
   TORCH_CHECK(out.dim() == 2 && out.size(0) == R && out.size(1) == hq * c.hd && out.stride(1) == 1 && aligned(out) &&
                   (R <= 1 || out.stride(0) % 8 == 0),
               "kv4.attention: out [sequences, q heads * head_dim], 16-byte aligned");
-  at::assert_no_internal_overlap(out);
+  if (out_given.has_value()) need_apart(out, "kv4.attention");
   rf::Kv4AttnArgs a{};
   if (gate.has_value()) {
     need(*gate, at::kBFloat16, c.pool, "gate");
