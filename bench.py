@@ -205,16 +205,11 @@ def decode_bench(args):
     rs = sorted({int(r) for r in args.decode.split(",") if r})
     if args.kv_bits == 4:                  # every cache in one pool of 4-bit pages, as the server with --kv-bits 4
         from ridgefill_data_b200.models.kvpool import KVPool
-        rows = args.decode_context + args.steps + 64
+        rows = args.decode_context + args.steps + 8
         model.kv_pool = KVPool(model, max(rs) * -(-rows // 128), 128, bits=4)
     g = torch.Generator().manual_seed(0)
-    caches, toks = [], []
-    with torch.no_grad():
-        for _ in range(max(rs)):
-            ids = torch.randint(0, cfg.vocab, (args.decode_context,), generator=g).to(device)
-            caches.append(run_lower(model, ids, [model.n_layers], reserve=args.steps + 64)[1])
-            toks.append(int(ids[-1]))
-    torch.cuda.synchronize()
+    prompts = [torch.randint(0, cfg.vocab, (args.decode_context,), generator=g).to(device) for _ in range(max(rs))]
+    toks = [int(ids[-1]) for ids in prompts]
     tensors = [t for w in model.W for t in w.values() if torch.is_tensor(t) and t.is_cuda]
     if torch.is_tensor(getattr(model, "lm_head", None)):
         tensors.append(model.lm_head)
@@ -230,8 +225,9 @@ def decode_bench(args):
     except (OSError, ValueError):
         pass
     for R in rs:
-        with torch.no_grad():
-            dg = DecodeGraph(model, caches[:R], headroom=args.steps + 8)
+        with torch.no_grad():              # caches of its own for every R: each is timed at --decode-context
+            caches = [run_lower(model, ids, [model.n_layers], reserve=args.steps + 64)[1] for ids in prompts[:R]]
+            dg = DecodeGraph(model, caches, headroom=args.steps + 8)
             for _ in range(3):
                 dg.step(toks[:R])
             torch.cuda.synchronize()
@@ -243,6 +239,10 @@ def decode_bench(args):
             torch.cuda.synchronize()
             ms = e0.elapsed_time(e1) / args.steps
             del dg
+            if args.kv_bits == 4:
+                for cache in caches:
+                    model.kv_pool.release(cache)
+            del caches
         print(json.dumps(dict(metric="greedy decode tokens/s (CUDA-graph step)", value=round(R * 1e3 / ms, 1),
                               unit="tokens/s", ms_per_step=round(ms, 3), sequences=R, steps=args.steps, warmup=3,
                               n_gpus=1, dtype="bf16", data="synthetic (seeded ids; random-init weights)",
