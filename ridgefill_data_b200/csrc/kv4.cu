@@ -4,7 +4,7 @@
 //                    (q, k), then q goes out in bf16 and k / v rows are quantised into their block.
 // kv4_append_rows_kernel  the same for many rows (below).
 // kv4_read_kernel    a block of 16 rows to shared memory in 16-byte pieces by 1, 2 or 4 warps, then 8 values a lane: the
-//                    numbers that the codes stand for, rounded once to bf16, whole rows to a store.
+//                    numbers that the codes stand for, in fp32 and from there in bf16, whole rows to a store.
 //
 // Roundings are the bf16 model's (norm and each step of the rotation round to bf16), so a cached key is the 4-bit form
 // of the row the bf16 cache would hold. The norm's sum of squares and its root are taken in 64 bits: products of two
@@ -384,11 +384,12 @@ __global__ void __launch_bounds__(256)
 //                       is written in place, row by row. The rotation's half is whole lanes (rot / 2 a multiple of 16).
 //
 // Both load the rows, the page's id and the rotation's entries before anything waits for one of them (80 -> 72 us for the
-// queries; behind one another each costs a trip to memory with 32 warps an SM to cover it). Bound by the instructions of the
-// cached rows (16 values of a lane: 190, 86 of them the codes) next to the queries' bytes. B200, 16384 rows: 32 q and 8 KV
-// heads of 128 74 us (356 MB: 54 at the measured 6.55 TB/s), the KV heads alone 37 (88 MB: 13.5); 24 gated and 4 of 256
-// with norms 109 us (491 MB: 75). Tried: row pieces through a ring of asynchronous copies (equal), the next wave's rows
-// fetched to L2 ahead (84 us), 3 CTAs an SM of 80 registers (82 us).
+// queries; behind one another each costs a trip to memory with 32 warps an SM to cover it). What is above the bytes is the
+// cached rows' arithmetic (16 values of a lane: 190 instructions, 86 of them the codes), a chain that 28 warps an SM do not
+// cover: issue slots 61 to 70 % busy, DRAM 30 to 58 %, so neither is at its limit. B200, 16384 rows: 32 q and 8 KV heads of
+// 128 72 us (356 MB: 54 at the measured 6.55 TB/s), the KV heads alone 35 (88 MB: 13.5); 24 gated and 4 of 256 with norms
+// 109 us (491 MB: 75). Tried: row pieces through a ring of asynchronous copies (equal), the next wave's rows fetched to L2
+// ahead (84 us), 3 CTAs an SM of 80 registers (82 us).
 
 // kept out of line: the common cases branch past it
 __device__ __noinline__ int divide(int a, int b) { return a / b; }
@@ -798,6 +799,9 @@ void launch_append(Kv4AppendArgs a, int r0, int seqs, cudaStream_t stream) {
   // From 256 rows on, in whole blocks' worth, the kernel for many rows; fewer: a warp a row and head, the shorter way through
   // a row. (32 + 8 heads of 128, many / few: 128 rows 3.5 / 3.3 us, 256 rows 4.1 / 4.7, 1024 rows 6.5 / 12.7; 16 sequences
   // of 8 rows 3.6 / 3.5, of 16 rows 3.9 / 5.0. 24 + 4 heads of 256 with norms: 256 rows 5.3 / 5.2, 1024 rows 10.0 / 12.7.)
+  // Rotary dims that are no multiple of 32 stay with a warp a row and head whatever the rows, since half of them is no whole
+  // number of the other kernel's lanes. (32 + 8 heads of 64 rotated over 16 / 32 dims: 1024 rows 12.2 / 4.9 us, 16384 rows
+  // 168 / 35.)
   if (a.T >= 16 && rows >= 256 && a.rot % 32 == 0) {
     switch ((a.norm_mode + 1) * 2 + (a.rot > 0)) {
       case 0: launch_rows<HD, -1, false>(a, r0, seqs, stream); break;

@@ -26,9 +26,7 @@ import torch
 
 from ._ext import ext
 
-BF16 = torch.bfloat16
 BLOCK = 16       # rows of a block
-GROUP = 32       # values that share a scale and a minimum
 
 
 def block_bytes(head_dim):
