@@ -321,6 +321,8 @@ def main():
                     help="nvls row-parallel products in this many row chunks, each chunk's GEMM beside the previous "
                          "chunk's all-reduce on a second stream (1: the fused GEMM + all-reduce kernel)")
     args = ap.parse_args()
+    if args.kv_bits != 16 and not args.decode:
+        ap.error("--kv-bits 4 times decode steps: give --decode")
     dsplit, dtail = DEFAULT_SPLIT_TAIL.get(args.model, (32, 4096))
     args.split = dsplit if args.split is None else args.split
     args.tail = dtail if args.tail is None else args.tail
