@@ -13,7 +13,9 @@ device and are read by the kernels, so a CUDA graph of these calls replays at ne
 or a row past the table records error code 7 (ops/_ext.py check_errors): append writes nothing there, read gives
 zeros, attention leaves the page's rows out (a position past the table: a zero row).
 
-Rows are independent: appending a row again overwrites it, rows not appended keep their bytes. Two sequences may share
+Rows are independent: appending a row again overwrites it, rows not appended keep their bytes; those of a new pool are zero
+rows, to read and to attention alike. A row's values are kept up to 2^56 (beyond that, or not finite, the whole row is NaN).
+Outputs given to a call must share no element. Two sequences may share
 pages that both only read; rows that one call, or two calls at once, append must be different rows of the pool. A
 sequence holds up to 2^30 rows. Head dims 64, 128 and 256.
 
