@@ -15,9 +15,8 @@ zeros, attention leaves the page's rows out (a position past the table: a zero r
 
 Rows are independent: appending a row again overwrites it, rows not appended keep their bytes; those of a new pool are zero
 rows, to read and to attention alike. A row's values are kept up to 2^56 (beyond that, or not finite, the whole row is NaN).
-Outputs given to a call must share no element. Two sequences may share
-pages that both only read; rows that one call, or two calls at once, append must be different rows of the pool. A
-sequence holds up to 2^30 rows. Head dims 64, 128 and 256.
+Outputs given to a call must share no element. Two sequences may share pages that both only read; rows that one call, or
+two calls at once, append must be different rows of the pool. A sequence holds up to 2^30 rows. Head dims 64, 128 and 256.
 
 A call works on the current stream and allocates what it needs for itself, so calls on several streams and captured graphs
 share nothing but the pool.
