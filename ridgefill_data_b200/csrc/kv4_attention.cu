@@ -216,6 +216,7 @@ struct QueryLoad {
 // Such rows get their own size in the ring before their block's values are used: large ones z below 2, s and m by a power
 // of two (exact, or to 2^-25 of a row of size 1), zeros the smallest size. So in every block P s <= 2^14 (4 / 15), and l
 // lies between 2^-56 and 2^54 a key. A marked row (255) misfits too and is left as it is.
+// Rows below 2^-40 count as of that size, as the cache holds them: from about 2^-50 on their P s loses bits.
 __device__ __forceinline__ bool size_misfits(int byte) { return (unsigned)(byte - (127 - kKv4Limit)) >= 2u * kKv4Limit; }
 
 template <int HD>
